@@ -165,6 +165,8 @@ int rhp_route_bwd(const void* dgates, const void* gates, const void* logits, con
  *   dx[t] = dout[t] + sum_j dxp[pair_row[t*k+j]] + sum_j dlogits_sel[t,j] * router_w[topi[t,j]]
  *           + sum_s shared_dx[s][t]
  * (residual + scatter-add of the permuted input gradient + router input gradient).
+ * dout may be NULL: no residual term (the layer behind a norm, whose residual
+ * passes the norm by).
  * dout, dxp, dx, shared_dx: dtype; dlogits_sel, router_w: r_dtype.
  */
 int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
@@ -421,6 +423,109 @@ int rhp_expert_fc1_dgrad_router(int G, const int32_t* offsets, int64_t rows_cap,
 int rhp_adam_step(int count, void* const* params, const void* const* grads, void* const* exp_avg,
                   void* const* exp_avg_sq, const int64_t* numel, int dtype, double lr, double beta1, double beta2,
                   double eps, double weight_decay, int64_t step, hipStream_t stream);
+
+/* ------------------------------------------------------------------ layer norm */
+
+/*
+ * Layer norm of T rows: y = (x - mean) * rstd * w + b with the row's mean and
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps), the normalisation in front of the
+ * pre-norm block (resihp/runtime/reference_model.py:195-234: out = x + f(norm(x))).
+ *   x, y: [T,h] dtype (F64/F32/BF16), contiguous; w, b: [h] w_dtype (the rows'
+ *   dtype, or F32 with BF16 rows), either may be NULL (ones, zeros); mean, rstd:
+ *   [T] float (double for F64 rows), what rhp_layer_norm_bwd takes.
+ * y must not overlap x.  Any 1 <= h <= 2^28, any T; rows need only their
+ * element's alignment.  A row's results depend on that row alone, whatever T.
+ */
+int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const void* b, int w_dtype, int64_t T, int h,
+                       double eps, void* y, void* mean, void* rstd, hipStream_t stream);
+
+/* Workspace bytes rhp_layer_norm_bwd needs for dw or db. */
+size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype);
+
+/*
+ * Its backward.  With g = dy * w and xh = (x - mean) * rstd:
+ *   dx[t] = rstd * (g - mean(g) - xh * mean(g * xh)) + dres[t]
+ *   dw    = sum over rows of dy * xh,  db = sum over rows of dy
+ * dres ([T,h] dtype, or NULL) is the gradient that reaches x beside the norm
+ * (the residual's).  dx may be NULL, dw and db ([h] w_dtype) too; what is NULL
+ * is not computed.  T == 0 writes zeros to dw and db.  Sums are float (double
+ * for F64 rows) in an order that the sizes fix.  dx may be dres; outputs must
+ * not overlap other inputs.  The workspace (16-byte aligned) is only needed
+ * with dw or db and holds nothing between calls.
+ */
+int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, const void* w, int w_dtype, const void* mean,
+                       const void* rstd, const void* dres, int64_t T, int h, void* dx, void* dw, void* db,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------ AdamW, gradient norm */
+
+/*
+ * Decoupled-decay Adam over many tensors in one launch, next to the
+ * reference's own Adam (rhp_adam_step):
+ *   g = gradient * *grad_scale
+ *   m = b1 m + (1 - b1) g,  v = b2 v + ((1 - b2) g) g
+ *   p = (1 - lr wd) p - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * in float (double for F64 weights), each weight rounded once.
+ *
+ * The tensors are described by a plan: rhp_adamw_plan writes an image of
+ * rhp_adamw_plan_bytes() bytes to host memory, the caller copies it to device
+ * memory (16-byte aligned) and gives both to every step.  Host arrays of
+ * `count` entries:
+ *   params: weights (F64/F32/BF16; F64 only among themselves); masters: F32
+ *   copies that BF16 weights are the rounded values of, or NULL (array or entry)
+ *   exp_avg, exp_avg_sq: F32 moments (F64 for F64 weights), or with state_bits = 8
+ *   one byte an element, with scales: [ceil(numel/128)][2] bytes
+ *   keys: what tells a tensor's random bits from the others' (state_bits = 8)
+ *   decay: 0 for tensors without weight decay (NULL: all decay)
+ * Tensors need their element's alignment.  The image holds addresses: a tensor
+ * that moves needs a new one.
+ *
+ * Moments in 8 bits (state_bits = 8): 128 neighbouring elements share an
+ * exponent byte E; a code is a float's exponent and three mantissa bits above
+ * the lowest binade the block keeps (m: sign + 7 bits, 16 binades; v: 8 bits,
+ * 32 binades): value = float_bits((code + 8 max(E - 15 | 31, 0)) << 20), code
+ * 0 = 0.  Rounding is stochastic with random bits from (seed, step, key,
+ * index): the same arguments give the same codes.  v > 0 never becomes 0.
+ * E = 255 marks a block with a value that is not finite: it reads as NaN.
+ */
+size_t rhp_adamw_plan_bytes(int count, const int64_t* numel);
+int rhp_adamw_plan(int count, void* const* params, const int* dtypes, void* const* masters, void* const* exp_avg,
+                   void* const* exp_avg_sq, void* const* scales, const int64_t* numel, const uint32_t* keys,
+                   const int* decay, int state_bits, void* image, size_t image_bytes);
+
+/*
+ * One step over a plan's tensors, in place.  grads: host array of device
+ * pointers (NULL array or entry: a gradient of zeros), g_dtypes their dtypes
+ * (F32 or BF16 whatever the weight's; F64 for F64 weights).  grad_scale:
+ * device float that every gradient is multiplied with (NULL: 1), read when the
+ * step runs.  step counts from 1.  The scalars are fixed when the call is
+ * enqueued, in a captured graph too.  One launch for up to 448 tensors.
+ */
+int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
+                   const int* g_dtypes, double lr, double beta1, double beta2, double eps, double weight_decay,
+                   int64_t step, const float* grad_scale, uint64_t seed, hipStream_t stream);
+
+/*
+ * The values that n codes stand for, as bfloat16 (which holds each exactly),
+ * and the codes nearest to n float moments.  scales: [ceil(n/128)][2] bytes.
+ */
+int rhp_moments_decode(const uint8_t* q_m, const uint8_t* q_v, const uint8_t* scales, int64_t n, void* m, void* v,
+                       hipStream_t stream);
+int rhp_moments_encode(const float* m, const float* v, int64_t n, uint8_t* q_m, uint8_t* q_v, uint8_t* scales,
+                       hipStream_t stream);
+
+/* Workspace bytes rhp_grad_norm needs for this many tensors. */
+size_t rhp_grad_norm_workspace_bytes(int count);
+
+/*
+ * out[0] = the 2-norm of all elements of the gradients, out[1] = min(1,
+ * max_norm / (out[0] + 1e-6)), what clips them (rhp_adamw_step's grad_scale).
+ * Summed in double: no square overflows, and the order is fixed.  A NaN or an
+ * infinity among the gradients makes the norm that, and the coefficient NaN or
+ * 0.  Gradients may mix F64/F32/BF16 and need their element's alignment.
+ */
+int rhp_grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel, double max_norm,
+                  float* out, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------ fp8 experts (delayed scaling) */
 

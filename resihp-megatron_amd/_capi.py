@@ -20,6 +20,7 @@ MAX_GROUPS_PER_LAUNCH = 64
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
+_u64 = ctypes.c_uint64
 _d = ctypes.c_double
 _sz = ctypes.c_size_t
 _pp = ctypes.POINTER(ctypes.c_void_p)
@@ -58,6 +59,16 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "rhp_expert_fc1_dgrad_scatter": (_i, [_i, _p, _i64, _i, _i, _i, _i, _p, _pp, _p, _i64, _p, _p, _sz, _p]),
     "rhp_expert_fc1_dgrad_router": (_i, [_i, _p, _i64, _i, _i, _i, _i, _pp, _pp, _p, _i, _p, _p, _pp, _p, _sz, _p]),
     "rhp_adam_step": (_i, [_i, _pp, _pp, _pp, _pp, _p, _i, _d, _d, _d, _d, _d, _i64, _p]),
+    "rhp_layer_norm_fwd": (_i, [_p, _i, _p, _p, _i, _i64, _i, _d, _p, _p, _p, _p]),
+    "rhp_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "rhp_layer_norm_bwd": (_i, [_p, _p, _i, _p, _i, _p, _p, _p, _i64, _i, _p, _p, _p, _p, _sz, _p]),
+    "rhp_adamw_plan_bytes": (_sz, [_i, _p]),
+    "rhp_adamw_plan": (_i, [_i, _pp, _p, _pp, _pp, _pp, _pp, _p, _p, _p, _i, _p, _sz]),
+    "rhp_adamw_step": (_i, [_p, _p, _sz, _pp, _p, _d, _d, _d, _d, _d, _i64, _p, _u64, _p]),
+    "rhp_moments_decode": (_i, [_p, _p, _p, _i64, _p, _p, _p]),
+    "rhp_moments_encode": (_i, [_p, _p, _i64, _p, _p, _p, _p]),
+    "rhp_grad_norm_workspace_bytes": (_sz, [_i]),
+    "rhp_grad_norm": (_i, [_i, _pp, _p, _p, _d, _p, _p, _sz, _p]),
     "rhp_fp8_padded_offsets": (_i, [_p, _i, _i, _p, _p]),
     "rhp_fp8_cast": (_i, [_p, _i, _i64, _i, _i, _p, _p, _i64, _p, _i, _i, _i, _p, _p, _p, _p, _p]),
     "rhp_fp8_cast_many": (_i, [_i, _pp, _pi64, _pi64, _pp, _i, _i, _i, _pp, _pp, _pp, _p]),

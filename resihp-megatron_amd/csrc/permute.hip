@@ -272,7 +272,12 @@ __global__ __launch_bounds__(kThreads) void token_bwd_kernel(const S* __restrict
         A acc[kChunksPerIter][8];
 #pragma unroll
         for (int u = 0; u < kChunksPerIter; ++u)
-            if (c0 + u * 64 < nch) Vec8<S, A>::load(dout + t * h + (c0 + u * 64) * 8, acc[u]);
+            if (dout) {
+                if (c0 + u * 64 < nch) Vec8<S, A>::load(dout + t * h + (c0 + u * 64) * 8, acc[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[u][i] = A(0);
+            }
         for (int j = 0; j < k; ++j) {
             if (rows[j] < 0) continue;
             A v[kChunksPerIter][8];
@@ -629,7 +634,7 @@ __device__ __forceinline__ void token_bwd_bf16_row(const bf16* __restrict__ dout
         uint4 dv[U], xv[KM][U], sv[SM > 0 ? SM : 1][U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c0 + u * 64 < nch) dv[u] = nt_load16(drow + (c0 + u * 64) * 8);
+            if (c0 + u * 64 < nch) dv[u] = dout ? nt_load16(drow + (c0 + u * 64) * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < KM; ++j)
             if (rows[j] >= 0) {
@@ -1068,7 +1073,7 @@ extern "C" int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* p
     if (int rc = check_rows("rhp_token_bwd", dtype, T, h, k)) return rc;
     RHP_REQUIRE(E >= 1 && n_shared >= 0 && n_shared <= kMaxShared, "rhp_token_bwd: bad E or n_shared");
     if (T == 0) return 0;
-    RHP_REQUIRE(dout && pair_row && topi && dx && aligned16(dout) && aligned16(dx),
+    RHP_REQUIRE(pair_row && topi && dx && aligned16(dout) && aligned16(dx),
                 "rhp_token_bwd: null or unaligned pointer");
     RHP_REQUIRE(dxp == nullptr || aligned16(dxp), "rhp_token_bwd: dxp must be 16-byte aligned");
     RHP_REQUIRE(dlogits_sel == nullptr || (router_w && aligned16(router_w)),

@@ -288,8 +288,10 @@ def combine_bwd(dout: torch.Tensor, y: torch.Tensor, gates: torch.Tensor, pair_r
 
 
 def token_bwd(dout: torch.Tensor, dxp: torch.Tensor | None, pair_row: torch.Tensor, dl: torch.Tensor | None,
-              topi: torch.Tensor, router_w: torch.Tensor, shared_dx: list[torch.Tensor] = ()) -> torch.Tensor:
-    """dx = dout + sum of the token's permuted-row gradients + router input gradient + shared gradients."""
+              topi: torch.Tensor, router_w: torch.Tensor, shared_dx: list[torch.Tensor] = (),
+              residual: bool = True) -> torch.Tensor:
+    """dx = dout + sum of the token's permuted-row gradients + router input gradient + shared gradients;
+    without ``residual`` the term dout is left out (a residual that does not pass through here)."""
     dev = _need_cuda(dout, dxp, pair_row, dl, topi, router_w, *shared_dx)
     T, h = dout.shape
     k = topi.shape[1]
@@ -303,7 +305,7 @@ def token_bwd(dout: torch.Tensor, dxp: torch.Tensor | None, pair_row: torch.Tens
         _expect(_rows_of(t, f"shared_dx[{i}]", h, dout.dtype) == T, "shared gradients need one row per token")
     dx = torch.empty_like(dout)
     arr = C.ptr_array([s.data_ptr() for s in shared_dx])
-    _call("rhp_token_bwd", dev, _ptr(dout), _ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi), _ptr(router_w),
+    _call("rhp_token_bwd", dev, _ptr(dout) if residual else None, _ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi), _ptr(router_w),
           dtype_code(router_w), arr, len(shared_dx), dtype_code(dout), T, h, router_w.shape[0], k, _ptr(dx))
     return dx
 
@@ -741,6 +743,216 @@ def adam_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], exp_
     _call("rhp_adam_step", dev, len(params), _arr(params), garr, _arr(exp_avg), _arr(exp_avg_sq), numel,
           dtype_code(params[0]), float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
           int(step))
+
+
+# ----------------------------------------------------------------------------- layer norm
+
+
+def _norm_args(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None) -> int:
+    """Checks a norm's rows and parameters; the code of the parameters' dtype."""
+    _expect(x.dim() == 2 and x.shape[1] >= 1, f"x must be [rows, h], got {tuple(x.shape)}")
+    dt = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _expect(tuple(t.shape) == (x.shape[1],), f"{name} must be [{x.shape[1]}], got {tuple(t.shape)}")
+            _expect(t.dtype == dt, "weight and bias must have one dtype")
+    _expect(dt == x.dtype or (x.dtype == torch.bfloat16 and dt == torch.float32),
+            f"weight and bias of {x.dtype} rows must be {x.dtype}" +
+            (" or float32" if x.dtype == torch.bfloat16 else "") + f", got {dt}")
+    dtype_code(x)
+    return dtype_code_of(dt)
+
+
+def _stat_dtype(x: torch.Tensor) -> torch.dtype:
+    return torch.float64 if x.dtype == torch.float64 else torch.float32
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Layer norm of the rows of ``x`` [T, h]: (y, mean [T], rstd [T]), the statistics in float32 (float64
+    for float64 rows), as ``layer_norm_bwd`` takes them.  ``weight`` and ``bias`` ([h]; x's dtype, or
+    float32 with bfloat16 rows) may be None."""
+    dev = _need_cuda(x, weight, bias)
+    wc = _norm_args(x, weight, bias)
+    T, h = x.shape
+    y = torch.empty_like(x)
+    mean, rstd = torch.empty(2, T, dtype=_stat_dtype(x), device=dev).unbind()
+    _call("rhp_layer_norm_fwd", dev, _ptr(x), dtype_code(x), _ptr(weight), _ptr(bias), wc, T, h, float(eps), _ptr(y),
+          _ptr(mean), _ptr(rstd))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, mean: torch.Tensor,
+                   rstd: torch.Tensor, dres: torch.Tensor | None = None, need_x: bool = True,
+                   need_weight: bool = True, need_bias: bool = True, dtype: torch.dtype | None = None
+                   ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients (dx, dweight, dbias) of ``layer_norm`` under ``dy``; ``dres`` is added to dx (the gradient
+    that reaches x beside the norm).  What is not needed is not computed and comes back as None.  dweight
+    and dbias have the weight's dtype (``dtype``, or x's, without a weight)."""
+    dev = _need_cuda(dy, x, weight, mean, rstd, dres)
+    wd = weight.dtype if weight is not None else x.dtype if dtype is None else dtype
+    wc = _norm_args(x, weight, None)
+    _expect(wd == x.dtype or (x.dtype == torch.bfloat16 and wd == torch.float32), f"no {wd} gradients of {x.dtype} rows")
+    T, h = x.shape
+    for name, t in (("dy", dy), ("dres", dres)):
+        if t is not None:
+            _expect(_rows_of(t, name, h, x.dtype) == T, f"{name} must have x's shape")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _expect(t.dtype == _stat_dtype(x) and tuple(t.shape) == (T,), f"{name} must be {_stat_dtype(x)} [{T}]")
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty(h, dtype=wd, device=dev) if need_weight else None
+    db = torch.empty(h, dtype=wd, device=dev) if need_bias else None
+    if not (need_x or need_weight or need_bias):
+        return None, None, None
+    ws_bytes = C.lib().rhp_layer_norm_bwd_workspace_bytes(T, h, dtype_code(x)) if need_weight or need_bias else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    _call("rhp_layer_norm_bwd", dev, _ptr(dy), _ptr(x), dtype_code(x), _ptr(weight), dtype_code_of(wd), _ptr(mean),
+          _ptr(rstd), _ptr(dres) if need_x else None, T, h, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
+    return dx, dw, db
+
+
+# ----------------------------------------------------------------------------- AdamW, gradient norm
+
+MOMENT_BLOCK = 128   # neighbouring elements that share an exponent, for moments in 8 bits
+
+
+def _int_array(kind, values) -> ctypes.Array:
+    return (kind * max(1, len(values)))(*values)
+
+
+class AdamWPlan:
+    """What an AdamW step needs to know of its tensors, laid out once (rhp_adamw_plan): the image on the host
+    and on the device, and the tensors themselves, which it keeps alive.
+
+    ``params`` are bfloat16 or float32 weights (or all float64); ``exp_avg`` and ``exp_avg_sq`` their
+    moments in float32 (float64), or, with ``scales`` (uint8 [ceil(numel / 128), 2] a tensor), in 8 bits
+    (uint8); ``masters`` float32 copies of bfloat16 weights, or None entries; ``keys`` tell the tensors'
+    random bits apart (8 bits); ``decay`` False exempts a tensor from weight decay."""
+
+    def __init__(self, params, exp_avg, exp_avg_sq, scales=None, masters=None, keys=None, decay=None):
+        n = len(params)
+        _expect(n > 0, "an AdamW plan needs a parameter")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise KernelArgumentError("an AdamW plan cannot be made while a graph is captured: step once before")
+        masters = [None] * n if masters is None else list(masters)
+        keys = [0] * n if keys is None else [int(k) & 0xFFFFFFFF for k in keys]
+        decay = [True] * n if decay is None else list(decay)
+        eight = scales is not None
+        scales = list(scales) if eight else [None] * n
+        _expect(n == len(exp_avg) == len(exp_avg_sq) == len(scales) == len(masters) == len(keys) == len(decay),
+                "one entry per parameter in every list")
+        self.device = _need_cuda(*params, *exp_avg, *exp_avg_sq, *scales, *masters)
+        for i, p in enumerate(params):
+            _expect(p.dtype in _DT, f"param {i}: unsupported dtype {p.dtype}")
+            st = torch.uint8 if eight else _stat_dtype(p)
+            for what, t in (("exp_avg", exp_avg[i]), ("exp_avg_sq", exp_avg_sq[i])):
+                _expect(t.dtype == st and t.shape == p.shape, f"{what} {i} must be {st} with the param's shape")
+            if eight:
+                want = (-(-p.numel() // MOMENT_BLOCK), 2)
+                _expect(scales[i] is not None and scales[i].dtype == torch.uint8 and tuple(scales[i].shape) == want,
+                        f"scales {i} must be uint8 {want}")
+            if masters[i] is not None:
+                _expect(masters[i].dtype == torch.float32 and masters[i].shape == p.shape,
+                        f"master {i} must be float32 with the param's shape")
+        self.params, self.tensors = list(params), (list(exp_avg), list(exp_avg_sq), scales, masters)
+        self.shapes = [p.shape for p in params]
+        self.dtypes = [p.dtype for p in params]
+        self.ptrs = [p.data_ptr() for p in params]
+        numel = _int_array(ctypes.c_int64, [p.numel() for p in params])
+        size = C.lib().rhp_adamw_plan_bytes(n, numel)
+        self.image = torch.empty(size, dtype=torch.uint8)
+        addr = lambda ts: C.ptr_array([0 if t is None else t.data_ptr() for t in ts])  # noqa: E731
+        C.call("rhp_adamw_plan", n, addr(params), _int_array(ctypes.c_int, [_DT[p.dtype] for p in params]),
+               addr(masters), addr(exp_avg), addr(exp_avg_sq), addr(scales) if eight else None, numel,
+               _int_array(ctypes.c_uint32, keys), _int_array(ctypes.c_int, [int(bool(d)) for d in decay]),
+               8 if eight else 32, self.image.data_ptr(), size)
+        self.dev_image = self.image.to(self.device)
+
+    def moved(self) -> bool:
+        """Whether a parameter's storage is no longer where the plan has it."""
+        return [p.data_ptr() for p in self.params] != self.ptrs
+
+
+def _grad_arrays(plan: AdamWPlan, grads):
+    """Pointer and dtype arrays of a plan's gradients, checked."""
+    _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
+    dev, ptrs, codes = plan.device.index, [], []
+    f64 = plan.dtypes[0] == torch.float64
+    for i, g in enumerate(grads):
+        if g is None:
+            ptrs.append(0)
+            codes.append(0)
+            continue
+        if g.get_device() != dev:
+            raise RuntimeError(f"gradient {i} is not on {plan.device}")
+        code = _DT.get(g.dtype)
+        _expect(code is not None and (code == C.F64) == f64, f"gradient {i} has dtype {g.dtype}")
+        _expect(g.shape == plan.shapes[i] and g.is_contiguous(), f"gradient {i} must be contiguous with the param's shape")
+        ptrs.append(g.data_ptr())
+        codes.append(code)
+    return C.ptr_array(ptrs), _int_array(ctypes.c_int, codes)
+
+
+def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
+               step: int, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
+    """One AdamW step over the plan's tensors, in place, in one launch (up to 448 tensors).
+
+    ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights); None steps with
+    zeros.  ``grad_scale``: float32 tensor of one element on the device that every gradient is multiplied
+    with.  ``step`` counts from 1.  ``seed``: of the random bits that round moments of 8 bits."""
+    garr, gcodes = _grad_arrays(plan, grads)
+    if plan.moved():
+        raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made")
+    if grad_scale is not None:
+        _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
+                f"grad_scale must be one float32 on {plan.device}")
+    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), garr,
+          gcodes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
+          _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)
+
+
+def _check_moments(q_m, q_v, scales) -> int:
+    n = q_m.numel()
+    _expect(q_m.dtype == q_v.dtype == scales.dtype == torch.uint8 and q_v.shape == q_m.shape,
+            "codes and scales must be uint8, both moments' codes of one shape")
+    want = (-(-n // MOMENT_BLOCK), 2)
+    _expect(tuple(scales.shape) == want, f"scales must be {want}, got {tuple(scales.shape)}")
+    return n
+
+
+def moments_decode(q_m: torch.Tensor, q_v: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values (m, v) that moments in 8 bits stand for, as bfloat16, which holds each exactly."""
+    dev = _need_cuda(q_m, q_v, scales)
+    n = _check_moments(q_m, q_v, scales)
+    m, v = (torch.empty(q_m.shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    _call("rhp_moments_decode", dev, _ptr(q_m), _ptr(q_v), _ptr(scales), n, _ptr(m), _ptr(v))
+    return m, v
+
+
+def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: torch.Tensor,
+                   scales: torch.Tensor) -> None:
+    """Writes the 8-bit codes nearest to float32 moments."""
+    dev = _need_cuda(m, v, q_m, q_v, scales)
+    n = _check_moments(q_m, q_v, scales)
+    _expect(m.dtype == v.dtype == torch.float32 and m.numel() == v.numel() == n, "m and v must be float32, one per code")
+    _call("rhp_moments_encode", dev, _ptr(m), _ptr(v), n, _ptr(q_m), _ptr(q_v), _ptr(scales))
+
+
+def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
+    """float32 [2] on the device: the 2-norm over all elements of all gradients (summed in float64), and
+    min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
+    one device, None entries skipped."""
+    grads = [g for g in grads if g is not None]
+    _expect(len(grads) > 0, "grad_norm needs a gradient")
+    _expect(max_norm > 0, "max_norm must be positive")
+    dev = _need_cuda(*grads)
+    codes = _int_array(ctypes.c_int, [dtype_code(g) for g in grads])
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    ws_bytes = C.lib().rhp_grad_norm_workspace_bytes(len(grads))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("rhp_grad_norm", dev, len(grads), C.ptr_array([g.data_ptr() for g in grads]), codes,
+          _int_array(ctypes.c_int64, [g.numel() for g in grads]), float(max_norm), _ptr(out), _ptr(ws), ws_bytes)
+    return out
 
 
 # ----------------------------------------------------------------------------- fp8 experts

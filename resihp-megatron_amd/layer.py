@@ -16,6 +16,7 @@ per-group pointers.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -45,6 +46,14 @@ class LayerMeta:
     @property
     def full(self) -> bool:
         return self.window == (0, self.num_experts)
+
+
+class Norm(NamedTuple):
+    """The layer norm in front of a pre-norm block (resihp/runtime/reference_model.py:195-234)."""
+
+    weight: torch.Tensor | None
+    bias: torch.Tensor | None
+    eps: float = 1e-5
 
 
 def _fc1_rows(act: str, f: int) -> int:
@@ -203,8 +212,8 @@ def _fc1_fwd(xs, offsets, rows_from_offsets: bool, rows_cap: int, fc1s, f: int, 
 
 class _MoELayerFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, meta: LayerMeta, opts, x, router_w, bias, *weights):
-        fp8, grad_mode = opts
+    def forward(ctx, meta: LayerMeta, opts, x, router_w, bias, norm_w, norm_b, *weights):
+        fp8, grad_mode, norm_eps = opts
         # Without a backward to come (no_grad, or no input that needs a gradient) fc1 writes only the
         # activation rows, and nothing is saved.
         keep = fp8 is not None or (grad_mode and any(ctx.needs_input_grad))
@@ -219,6 +228,10 @@ class _MoELayerFn(torch.autograd.Function):
         shared_off = shared_h = shared_a = shared_y = None
         K.need_device(x, router_w, fc1s, fc2s, sfc1s, sfc2s)
         main = torch.cuda.current_stream(x.device)
+        # Behind a norm the layer works on its output; x itself is only the residual.
+        res, mean, rstd = x, None, None
+        if norm_eps is not None:
+            x, mean, rstd = K.layer_norm(res, norm_w, norm_b, norm_eps)
         # Shared experts need only x: concurrently with the routing and the routed experts on a side
         # stream where the products run concurrently, else after them.
         shared_side = S > 0 and T > 0 and _concurrent(h, _fc1_rows(meta.act, fs))
@@ -259,15 +272,16 @@ class _MoELayerFn(torch.autograd.Function):
             K.expert_fc2_fwd(shared_a, shared_off, False, T, sfc2s, shared_y)
         if shared_side:
             main.wait_stream(_side_stream(x.device))
-        out = K.combine(y, x, gates, topi, plan.pair_row, shared_y or [])
+        out = K.combine(y, res, gates, topi, plan.pair_row, shared_y or [])
         ctx.mark_non_differentiable(plan.counts)
         if not keep:
             return out, plan.counts
         ctx.meta = meta
         ctx.fp8 = (fp8, q8)
+        ctx.norm_dtype = None if norm_b is None else norm_b.dtype
         ctx.dims = (T, h, P, G, S)
         ctx.save_for_backward(x, router_w, logits, topi, gates, plan.perm, plan.offsets, plan.pair_row, xp, hpre,
-                              act, y, *weights)
+                              act, y, *weights, *(() if mean is None else (res, norm_w, mean, rstd)))
         ctx.shared = (shared_off, shared_h, shared_a)
         return out, plan.counts
 
@@ -276,13 +290,17 @@ class _MoELayerFn(torch.autograd.Function):
         meta = ctx.meta
         T, h, P, G, S = ctx.dims
         (x, router_w, logits, topi, gates, perm, offsets, pair_row, xp, hpre, act, y, *ws) = ctx.saved_tensors
+        normed = len(ws) > 2 * (G + S)
+        if normed:
+            *ws, res, norm_w, mean, rstd = ws
         fc1s, fc2s = ws[:G], ws[G:2 * G]
         sfc1s, sfc2s = ws[2 * G:2 * G + S], ws[2 * G + S:]
         shared_off, shared_h, shared_a = ctx.shared
         f = meta.ffn
         fs = meta.shared_ffn or f
         dout = dout.contiguous()
-        need_x = ctx.needs_input_grad[2]
+        need_norm = ctx.needs_input_grad[5:7]
+        need_x = ctx.needs_input_grad[2] or any(need_norm)
         main = torch.cuda.current_stream(x.device)
         sdw1 = [torch.empty_like(w) for w in sfc1s]
         sdw2 = [torch.empty_like(w) for w in sfc2s]
@@ -340,11 +358,44 @@ class _MoELayerFn(torch.autograd.Function):
                             [x] * S, shared_dx or None, sdw1, sdw2)
         if shared_side:
             main.wait_stream(_side_stream(x.device))
-        dx = K.token_bwd(dout, dxp, pair_row, None if fold else dl, topi, router_w, shared_dx) if need_x else None
+        dx = K.token_bwd(dout, dxp, pair_row, None if fold else dl, topi, router_w, shared_dx,
+                         residual=not normed) if need_x else None
+        dnw = dnb = None
+        if normed and need_x:
+            dx, dnw, dnb = K.layer_norm_bwd(dx, res, norm_w, mean, rstd, dres=dout, need_x=ctx.needs_input_grad[2],
+                                            need_weight=need_norm[0], need_bias=need_norm[1], dtype=ctx.norm_dtype)
         if dwr is not None:
             main.wait_stream(_side_stream(x.device))
             dwr.record_stream(main)   # made on the side stream, used on the caller's
-        return (None, None, dx, dwr, None, *dw1, *dw2, *sdw1, *sdw2)
+        return (None, None, dx, dwr, None, dnw, dnb, *dw1, *dw2, *sdw1, *sdw2)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, eps, x, weight, bias):
+        y, mean, rstd = K.layer_norm(x, weight, bias, eps)
+        ctx.norm_dtype = None if bias is None else bias.dtype
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        _, need_x, need_w, need_b = ctx.needs_input_grad
+        return None, *K.layer_norm_bwd(dy.contiguous(), x, weight, mean, rstd, need_x=need_x, need_weight=need_w,
+                                       need_bias=need_b, dtype=ctx.norm_dtype)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of ``x`` (with autograd), in float32 (float64 for float64) whatever
+    x's dtype.  ``weight`` and ``bias``: [h] in x's dtype, or float32 with bfloat16 rows, or None."""
+    h = x.shape[-1]
+    if h == 0:
+        raise K.KernelArgumentError("layer_norm needs at least one element a row")
+    rows = x.reshape(-1, h).contiguous()
+    return _LayerNormFn.apply(float(eps), rows, None if weight is None else weight.contiguous(),
+                              None if bias is None else bias.contiguous()).view(x.shape)
 
 
 class _ExpertChunksFn(torch.autograd.Function):
@@ -452,8 +503,12 @@ def expert_chunks(recv: torch.Tensor, recv_counts: torch.Tensor, fc1s: list[torc
 
 def moe_layer(meta: LayerMeta, x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None,
               fc1s: list[torch.Tensor], fc2s: list[torch.Tensor], shared_fc1s: list[torch.Tensor] = (),
-              shared_fc2s: list[torch.Tensor] = (), fp8: Fp8State | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+              shared_fc2s: list[torch.Tensor] = (), fp8: Fp8State | None = None,
+              norm: Norm | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Layer output and the int32 per-expert counts (``counts[E]`` counts invalid ids).
+
+    With ``norm`` the layer is a pre-norm block: it routes and computes on layer_norm(x), and x itself is
+    the residual; the backward adds the residual's gradient inside the norm's.
 
     With ``fp8`` the routed experts run in fp8 (e4m3 weights and activations, e5m2 gradients) with the
     delayed scaling of that state; the caller ends each iteration with ``fp8.finish_iteration()``.
@@ -471,6 +526,8 @@ def moe_layer(meta: LayerMeta, x: torch.Tensor, router_w: torch.Tensor, bias: to
         raise ValueError(f"need one fc1 and one fc2 weight per local expert ({e1 - e0})")
     if len(shared_fc1s) != meta.num_shared or len(shared_fc2s) != meta.num_shared:
         raise ValueError(f"need {meta.num_shared} shared expert weight pairs")
-    return _MoELayerFn.apply(meta, (fp8, torch.is_grad_enabled()), x.contiguous(), router_w.contiguous(),
-                             None if bias is None else bias.detach().contiguous(),
-                             *fc1s, *fc2s, *shared_fc1s, *shared_fc2s)
+    norm_w, norm_b, eps = (None, None, None) if norm is None else norm
+    return _MoELayerFn.apply(meta, (fp8, torch.is_grad_enabled(), None if eps is None else float(eps)), x.contiguous(),
+                             router_w.contiguous(), None if bias is None else bias.detach().contiguous(),
+                             None if norm_w is None else norm_w.contiguous(),
+                             None if norm_b is None else norm_b.contiguous(), *fc1s, *fc2s, *shared_fc1s, *shared_fc2s)

@@ -27,11 +27,12 @@ from __future__ import annotations
 
 import zlib
 from dataclasses import dataclass
+from types import MappingProxyType
 
 import torch
 
 from . import kernels as K
-from .layer import LayerMeta, expert_chunks, moe_layer
+from .layer import LayerMeta, Norm, expert_chunks, layer_norm, moe_layer
 from .placement import ExpertPlacement, expert_dp_groups, send_tables
 from .rng import generator
 from .state import FULL, GroupSpec, Holdings, TensorSpec
@@ -60,6 +61,8 @@ class MoEConfig:
     init_std: float = 0.0           # weights N(0, std) (0 -> N(0, 1/fan_in) as the reference)
     router_dtype: torch.dtype | None = None   # None -> float64 for float64 models, else float32
     device: str = "cuda"
+    norm: str = "none"              # "layer": a pre-norm block, out = x + moe(layer_norm(x))
+    norm_eps: float = 1e-5
 
 
 def router_dtype(cfg: MoEConfig) -> torch.dtype:
@@ -72,15 +75,32 @@ def _has_bias(cfg: MoEConfig) -> bool:
     return bool(cfg.bias_update_rate) or cfg.expert_bias
 
 
+NORM_KEYS = ("norm.weight", "norm.bias")
+
+
+def _has_norm(cfg: MoEConfig) -> bool:
+    if cfg.norm not in ("none", "layer"):
+        raise ValueError(f"norm must be 'none' or 'layer', not {cfg.norm!r}")
+    return cfg.norm == "layer"
+
+
+def _norm(cfg: MoEConfig, params: dict[str, torch.Tensor]) -> Norm | None:
+    return Norm(params["norm.weight"], params["norm.bias"], cfg.norm_eps) if _has_norm(cfg) else None
+
+
 def _fc1_rows(cfg: MoEConfig, ffn: int) -> int:
     return 2 * ffn if cfg.act == "swiglu" else ffn
 
 
 def moe_specs(cfg: MoEConfig) -> dict[str, TensorSpec]:
     """State contract (moe.py:42-50).  SwiGLU keeps ``experts.{e}.fc1.weight`` with 2*ffn rows
-    (gate rows first); shared experts are ``shared_experts.{s}.*`` and replicated like the router."""
+    (gate rows first); shared experts are ``shared_experts.{s}.*`` and replicated like the router, as are
+    a pre-norm block's ``norm.weight`` and ``norm.bias`` (in the router's dtype)."""
     h, f = cfg.hidden, cfg.ffn
     out = {"router.weight": TensorSpec("router.weight", (cfg.num_experts, h), None)}
+    if _has_norm(cfg):
+        for key in NORM_KEYS:
+            out[key] = TensorSpec(key, (h,), None)
     if _has_bias(cfg):
         out["router.expert_bias"] = TensorSpec("router.expert_bias", (cfg.num_experts,), None, trainable=False)
     for e in range(cfg.num_experts):
@@ -99,12 +119,15 @@ def expert_of(key: str) -> int | None:
 
 
 def _param_dtype(cfg: MoEConfig, key: str) -> torch.dtype:
-    return router_dtype(cfg) if key.startswith("router.") else cfg.dtype
+    return router_dtype(cfg) if key.startswith(("router.", "norm.")) else cfg.dtype
 
 
 def init_param(cfg: MoEConfig, spec: TensorSpec) -> torch.Tensor:
-    """moe.py:57-61: randn(gen(seed, crc32(key))) / sqrt(fan_in), drawn on the CPU, then moved."""
+    """moe.py:57-61: randn(gen(seed, crc32(key))) / sqrt(fan_in), drawn on the CPU, then moved.  A norm
+    starts as ones and zeros."""
     dt = _param_dtype(cfg, spec.key)
+    if spec.key in NORM_KEYS:
+        return torch.full(spec.global_shape, float(spec.key == "norm.weight"), dtype=dt, device=cfg.device)
     gen_dt = torch.float64 if dt == torch.float64 else torch.float32
     if not spec.trainable:
         if not cfg.bias_init_std:
@@ -200,7 +223,8 @@ def reference_forward(cfg: MoEConfig, params: dict[str, torch.Tensor], x: torch.
     """moe.py:90-101: route, in-forward bias update from this batch's loads, experts, combine + residual."""
     bias = params.get("router.expert_bias")
     fc1s, fc2s, s1, s2 = _weights(cfg, params, range(cfg.num_experts))
-    out, counts = moe_layer(_layer_meta(cfg), x, params["router.weight"], bias, fc1s, fc2s, s1, s2)
+    out, counts = moe_layer(_layer_meta(cfg), x, params["router.weight"], bias, fc1s, fc2s, s1, s2,
+                            norm=_norm(cfg, params))
     if bias is not None and cfg.bias_update_rate:
         K.update_expert_bias(bias, counts[: cfg.num_experts].contiguous(), cfg.bias_update_rate)
     return out
@@ -250,6 +274,149 @@ class Adam:
                 p.data.copy_(tensors[f"param/{n}"])
                 self.state[n]["exp_avg"].copy_(tensors[f"exp_avg/{n}"])
                 self.state[n]["exp_avg_sq"].copy_(tensors[f"exp_avg_sq/{n}"])
+        self.step_count = step_count
+
+
+class AdamW:
+    """Name-keyed AdamW over bfloat16 and float32 (or float64) parameters, one launch a step: decoupled
+    weight decay, moments in float32 (float64 for float64 parameters) whatever the parameters' type, or in 8
+    bits, and the gradients clipped to a global norm without a host synchronisation.  No counterpart in the
+    reference, whose Adam (resihp/runtime/optim.py:15-62) is ``Adam``; the interface is that class's.
+
+    ``state_bits``: 32, or 8 (a byte an element and moment and two bytes a block of 128, stochastically
+    rounded: ``seed``, the step and the parameter's name give the random bits, so a run is reproducible and
+    a parameter keeps its own when it moves).  ``master_weights``: float32 masters of the bfloat16
+    parameters, which are then the masters' rounded values.  ``max_grad_norm``: clips; ``grad_norm`` then
+    holds the last step's [norm, coefficient] on the device.  ``no_decay``: names without weight decay.
+
+    The state lives in a few flat buffers (``buffers()``), each tensor from a multiple of 128 elements on,
+    in the order of ``params``; ``state_tensors()`` names views of it.
+    """
+
+    def __init__(self, params: dict[str, torch.nn.Parameter], lr: float = 1e-3, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32, master_weights: bool = False,
+                 max_grad_norm: float | None = None, no_decay=(), seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"the moments have 32 or 8 bits, not {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError("max_grad_norm must be positive")
+        if any(n not in params for n in no_decay):
+            raise ValueError(f"no_decay names no parameter: {[n for n in no_decay if n not in params]}")
+        for n, p in params.items():
+            if not p.is_cuda:
+                raise RuntimeError(f"AdamW: parameter {n} is not on a HIP device; the fused step runs on the GPU")
+        self.params = dict(params)
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.state_bits, self.max_grad_norm, self.no_decay, self.seed = state_bits, max_grad_norm, set(no_decay), seed
+        self.step_count = 0
+        self.grad_norm: torch.Tensor | None = None
+        f64 = [n for n, p in self.params.items() if p.dtype == torch.float64]
+        if f64 and (len(f64) < len(self.params) or state_bits == 8):
+            raise ValueError("float64 parameters need an AdamW of their own, with 32-bit (here float64) moments")
+        self._flat: dict[str, torch.Tensor] = {}
+        if not self.params:
+            return
+        names = list(self.params)
+        state = torch.uint8 if state_bits == 8 else torch.float64 if f64 else torch.float32
+        self.state = {n: {} for n in names}
+        for key in ("exp_avg", "exp_avg_sq"):
+            self._allocate(key, names, state)
+        if state_bits == 8:
+            blocks = [-(-self.params[n].numel() // K.MOMENT_BLOCK) for n in names]
+            flat = torch.zeros(sum(blocks), 2, dtype=torch.uint8, device=self.params[names[0]].device)
+            self._flat["scales"] = flat
+            for n, t in zip(names, flat.split(blocks)):
+                self.state[n]["scales"] = t
+        if master_weights:
+            low = [n for n in names if self.params[n].dtype == torch.bfloat16]
+            if low:
+                self._allocate("master", low, torch.float32)
+            for n in low:
+                self.state[n]["master"].copy_(self.params[n].detach())
+        # Read-only: the step knows the buffers, a tensor put in a view's place would not be seen.
+        self.state = {n: MappingProxyType(t) for n, t in self.state.items()}
+        self._plan: K.AdamWPlan | None = None
+
+    def _allocate(self, key: str, names: list[str], dtype: torch.dtype) -> None:
+        sizes = [self.params[n].numel() for n in names]
+        padded = [-(-k // K.MOMENT_BLOCK) * K.MOMENT_BLOCK for k in sizes]
+        flat = torch.zeros(sum(padded), dtype=dtype, device=self.params[names[0]].device)
+        self._flat[key] = flat
+        for n, k, t in zip(names, sizes, flat.split(padded)):
+            self.state[n][key] = t[:k].view(self.params[n].shape)
+
+    def zero_grad(self) -> None:
+        for p in self.params.values():
+            p.grad = None
+
+    @torch.no_grad()
+    def step(self) -> None:
+        """One step from the parameters' gradients (None: a gradient of zeros, as ``Adam`` has it)."""
+        if not self.params:
+            self.step_count += 1
+            return
+        grads = [p.grad for p in self.params.values()]
+        plan = self._plan
+        if plan is None or plan.moved():
+            plan = self._plan = self._make_plan()
+        norm = None
+        if self.max_grad_norm is not None and any(g is not None for g in grads):
+            norm = K.grad_norm(grads, self.max_grad_norm)
+        K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
+                     None if norm is None else norm[1:], self.seed)
+        self.step_count += 1
+        self.grad_norm = norm
+
+    def _make_plan(self) -> K.AdamWPlan:
+        names = list(self.params)
+        of = lambda key: [self.state[n].get(key) for n in names]  # noqa: E731
+        return K.AdamWPlan([self.params[n] for n in names], of("exp_avg"), of("exp_avg_sq"),
+                           of("scales") if self.state_bits == 8 else None, of("master"),
+                           [zlib.crc32(n.encode()) for n in names], [n not in self.no_decay for n in names])
+
+    def buffers(self) -> dict[str, torch.Tensor]:
+        """The flat buffers that hold the state: "exp_avg", "exp_avg_sq", and where there are any "scales"
+        and "master"."""
+        return dict(self._flat)
+
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Both moments' values as flat buffers (bfloat16, exactly, where they are held in 8 bits)."""
+        if self.state_bits == 8:
+            return K.moments_decode(self._flat["exp_avg"], self._flat["exp_avg_sq"], self._flat["scales"])
+        return self._flat["exp_avg"], self._flat["exp_avg_sq"]
+
+    def state_tensors(self) -> dict[str, torch.Tensor]:
+        out: dict[str, torch.Tensor] = {}
+        for n, p in self.params.items():
+            out[f"param/{n}"] = p.data
+            for key, t in self.state[n].items():
+                out[f"{key}/{n}"] = t
+        return out
+
+    @torch.no_grad()
+    def load_state_tensors(self, tensors: dict[str, torch.Tensor], step_count: int) -> None:
+        """Copies a state in.  Float moments load into 8 bits as the nearest codes, 8-bit ones into float32
+        as their values; without masters, masters start from the parameters."""
+        for n, p in self.params.items():
+            p.data.copy_(tensors[f"param/{n}"])
+            m, v, sc = (tensors.get(f"{key}/{n}") for key in ("exp_avg", "exp_avg_sq", "scales"))
+            if m is None or v is None:
+                raise KeyError(f"no moments of {n}")
+            mine = self.state[n]
+            if (m.dtype == torch.uint8) != (self.state_bits == 8):
+                m, v = (t.to(p.device) for t in (m, v))
+                if self.state_bits == 8:
+                    K.moments_encode(m.float().contiguous(), v.float().contiguous(), mine["exp_avg"],
+                                     mine["exp_avg_sq"], mine["scales"])
+                else:
+                    m, v = K.moments_decode(m.contiguous(), v.contiguous(), sc.to(p.device).contiguous())
+            if self.state_bits == 32 or m.dtype == torch.uint8:
+                mine["exp_avg"].copy_(m)
+                mine["exp_avg_sq"].copy_(v)
+                if self.state_bits == 8:
+                    mine["scales"].copy_(sc)
+            if "master" in mine:
+                mine["master"].copy_(tensors.get(f"master/{n}", p.data))
         self.step_count = step_count
 
 
@@ -352,7 +519,8 @@ class EPRuntime:
             raise RuntimeError(f"{self.me} received tokens for expert {missing[0]} it does not host")
         fc1s, fc2s, s1, s2 = _weights(cfg, self.params, range(E))
         out, counts = moe_layer(_layer_meta(cfg), x, self.params["router.weight"],
-                                self.buffers.get("router.expert_bias"), fc1s, fc2s, s1, s2)
+                                self.buffers.get("router.expert_bias"), fc1s, fc2s, s1, s2,
+                                norm=_norm(cfg, self.params))
         self.tokens_per_expert = counts[:E].to(torch.float64)
         return out
 
@@ -373,9 +541,13 @@ class EPRuntime:
         gates)``: ``rows`` [P, h] = ``x.index_select(0, idx_i)`` in send order (:212), ``counts``
         the ``[|ep|, E]`` int64 matrix exchanged first (:199-209), ``in_splits`` its row sums
         (:210), the ``K.SendPlan`` (``plan.row`` is the pair -> row map the combine of the
-        returned rows takes, :225-226) and the gates.  Sets ``tokens_per_expert`` like forward."""
+        returned rows takes, :225-226) and the gates.  Sets ``tokens_per_expert`` like forward.  In a
+        pre-norm block the normalised rows are routed and sent; the combine's residual is ``x`` itself."""
         cfg, E = self.cfg, self.cfg.num_experts
         bias = self.buffers.get("router.expert_bias")
+        norm = _norm(cfg, self.params)
+        if norm is not None:
+            x = K.layer_norm(x.detach().contiguous(), norm.weight.detach(), norm.bias.detach(), norm.eps)[0]
         _, topi, gates = K.route(x.detach().contiguous(), self.params["router.weight"].detach().contiguous(),
                                  None if bias is None else bias.detach().contiguous(), cfg.top_k, cfg.score,
                                  cfg.normalize, cfg.gate_scale)
@@ -437,5 +609,5 @@ class EPRuntime:
 
 
 __all__ = ["MoEConfig", "moe_specs", "expert_of", "init_param", "update_expert_bias", "batch", "route", "expert_ffn",
-           "token_loss", "reference_forward", "reference_train", "moe_holdings", "edp_group_name", "moe_group_specs",
-           "EPRuntime", "local_keys", "Adam", "even_split"]
+           "token_loss", "reference_forward", "reference_train", "moe_holdings", "edp_group_name", "moe_group_specs", "layer_norm",
+           "EPRuntime", "local_keys", "Adam", "AdamW", "even_split"]
