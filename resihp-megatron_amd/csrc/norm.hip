@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "rhp_common.h"
 
@@ -47,6 +48,8 @@ template <class A> __device__ __forceinline__ A block_sum(A v, A* s) {
     __syncthreads();
     return t;
 }
+
+// ------------------------------------------------------------------ rows of any length
 
 // One block a row, any h: the row is read three times, the last two from the caches.
 template <class S, class W>
@@ -143,16 +146,332 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_cols_kernel(
     }
 }
 
-// dw, db = the sum of the slices' partial sums.
+// dw, db = the sums of the partial rows, a column a lane: 16 waves each sum every 16th, then wave 0 their sums.
+constexpr int kReduceThreads = 1024;
 template <class A, class W>
-__global__ __launch_bounds__(kNormThreads) void norm_bwd_reduce_kernel(const A* __restrict__ part, int slices, int h,
-                                                                       W* __restrict__ dw, W* __restrict__ db) {
-    const int i = blockIdx.x * kNormThreads + threadIdx.x;
-    if (i >= 2 * h) return;
+__global__ __launch_bounds__(kReduceThreads) void norm_bwd_reduce_kernel(const A* __restrict__ part, int parts, int h,
+                                                                         W* __restrict__ dw, W* __restrict__ db) {
+    constexpr int kWaves = kReduceThreads / 64;
+    __shared__ A s[kWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     A sum = 0;
-    for (int s = 0; s < slices; ++s) sum += part[static_cast<int64_t>(s) * 2 * h + i];
+    if (i < 2 * static_cast<int64_t>(h)) {
+#pragma unroll 4
+        for (int k = wave; k < parts; k += kWaves) sum += part[static_cast<int64_t>(k) * 2 * h + i];
+    }
+    s[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || i >= 2 * static_cast<int64_t>(h)) return;
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) sum += s[k][lane];
     W* out = i < h ? dw : db;
     if (out) Elem<W>::st(out, i < h ? i : i - h, sum);
+}
+
+// ------------------------------------------------------------------ rows in registers
+
+// Rows of up to 2 x 16 bytes for each of up to 1024 threads are read once and
+// held in registers: TPR threads (whole waves) own a row, each of them two
+// chunks of 16 bytes, TPR * 16 bytes apart.  The blocks stay and walk the rows;
+// the next row's loads are in flight while this one is reduced, and the weight
+// (and, in the backward, the columns' sums of dw and db) stay in registers from
+// row to row.
+//
+// Rows that end inside a chunk (kTail): the last chunk is the row's last 16
+// bytes, so it overlaps the one before it.  Its first `dup` elements count for
+// no sum; both threads store the same bits to them.  A vector access needs no
+// alignment beyond its element's.
+typedef uint32_t Q __attribute__((ext_vector_type(4)));
+typedef Q Qu __attribute__((aligned(2)));
+constexpr int kChunks = 2;
+
+template <class S> constexpr int kVec = 16 / static_cast<int>(sizeof(S));
+
+template <class S> struct Chunk {
+    Q q;
+    __device__ __forceinline__ void load(const S* p) { q = __builtin_nontemporal_load(reinterpret_cast<const Qu*>(p)); }
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(S) == 4) return __uint_as_float(q[j]);
+        return __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
+    }
+};
+template <class S> __device__ __forceinline__ void store_chunk(S* p, const float* v) {
+    Q q;
+    if constexpr (sizeof(S) == 4)
+        q = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else
+        q = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    *reinterpret_cast<Qu*>(p) = q;
+}
+// N parameters from p on (every block reads them once: the ordinary cache policy).
+template <int N, class W> __device__ __forceinline__ void load_params(const W* p, float* v) {
+    constexpr int M = kVec<W>;
+#pragma unroll
+    for (int k = 0; k < N; k += M) {
+        Chunk<W> c;
+        if constexpr (M <= N) {
+            c.q = *reinterpret_cast<const Qu*>(p + k);
+#pragma unroll
+            for (int j = 0; j < M; ++j) v[k + j] = c.at(j);
+        }
+    }
+}
+
+// Where a thread's chunks lie: first element, how many of its first elements
+// another chunk counts, whether it has any.
+template <int N, int TPR, bool kTail> struct Place {
+    int off[kChunks], dup[kChunks];
+    bool on[kChunks];
+    __device__ __forceinline__ Place(int i, int h) {
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v) {
+            const int c = (i + v * TPR) * N;
+            on[v] = c < h;
+            off[v] = kTail ? min(c, h - N) : c;
+            dup[v] = c - off[v];
+        }
+    }
+    __device__ __forceinline__ bool counts(int v, int j) const { return !kTail || j >= dup[v]; }
+};
+
+// Sums of K values over the TPR threads of a row, in all of them.  `s` has a
+// slot a wave; a call and the next one use different slots, so one barrier a
+// call is enough.
+template <int K, int TPR> __device__ __forceinline__ void row_sums(float (&v)[K], float (*s)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) s[wave][k] = v[k];
+        __syncthreads();
+        const int w0 = wave / (TPR / 64) * (TPR / 64);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            v[k] = s[w0][k];
+#pragma unroll
+            for (int i = 1; i < TPR / 64; ++i) v[k] += s[w0 + i][k];
+        }
+    }
+}
+
+constexpr int fwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int bwd_threads(int tpr) { return tpr < 512 ? 512 : tpr; }
+constexpr int kFwdBlocksPerCu = 4;   // of 256 threads
+
+template <class S, class W, int TPR, bool kTail>
+__global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S* __restrict__ x,
+                                                                        const W* __restrict__ w,
+                                                                        const W* __restrict__ b, int64_t T, int h,
+                                                                        float eps, S* __restrict__ y,
+                                                                        float* __restrict__ mean,
+                                                                        float* __restrict__ rstd) {
+    constexpr int N = kVec<S>, G = fwd_threads(TPR) / TPR;
+    __shared__ float red[2][fwd_threads(TPR) / 64][1];
+    const int grp = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / TPR));
+    const Place<N, TPR, kTail> at(threadIdx.x % TPR, h);
+    float wv[kChunks][N], bv[kChunks][N];
+    Chunk<S> cur[kChunks], nxt[kChunks];
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * G;
+    int64_t t = static_cast<int64_t>(blockIdx.x) * G + grp;
+#pragma unroll
+    for (int v = 0; v < kChunks; ++v) {
+        cur[v].q = Q{0, 0, 0, 0};
+        if (at.on[v] && t < T) cur[v].load(x + t * h + at.off[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < kChunks; ++v) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            wv[v][j] = 1.0f;
+            bv[v][j] = 0.0f;
+        }
+        if (w && at.on[v]) load_params<N>(w + at.off[v], wv[v]);
+        if (b && at.on[v]) load_params<N>(b + at.off[v], bv[v]);
+    }
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < T; base += stride, t += stride) {
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v) {
+            nxt[v].q = Q{0, 0, 0, 0};
+            if (at.on[v] && t + stride < T) nxt[v].load(x + (t + stride) * h + at.off[v]);
+        }
+        float sum[1] = {0.0f}, sq[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v)
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[0] += at.counts(v, j) ? cur[v].at(j) : 0.0f;
+        row_sums<1, TPR>(sum, red[0]);
+        const float mu = sum[0] / static_cast<float>(h);
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v)
+            if (at.on[v]) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float d = cur[v].at(j) - mu;
+                    sq[0] += at.counts(v, j) ? d * d : 0.0f;
+                }
+            }
+        row_sums<1, TPR>(sq, red[1]);
+        const float r = rsqrt_t(sq[0] / static_cast<float>(h) + eps);
+        if (t < T) {
+#pragma unroll
+            for (int v = 0; v < kChunks; ++v)
+                if (at.on[v]) {
+                    float o[N];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) o[j] = (cur[v].at(j) - mu) * r * wv[v][j] + bv[v][j];
+                    store_chunk(y + t * h + at.off[v], o);
+                }
+            if (threadIdx.x % TPR == 0) {
+                mean[t] = mu;
+                rstd[t] = r;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v) cur[v] = nxt[v];
+    }
+}
+
+constexpr int kNormMaxParts = 256;   // partial sums of dw and db (blocks of the backward): one a CU
+
+template <class S> struct BwdRow {
+    Chunk<S> x[kChunks], dy[kChunks], res[kChunks];
+    float mu, r;
+};
+
+template <class S, class W, int TPR, bool kTail, bool kSums>
+__global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
+    const S* __restrict__ dy, const S* __restrict__ x, const W* __restrict__ w, const float* __restrict__ mean,
+    const float* __restrict__ rstd, const S* __restrict__ dres, int64_t T, int h, S* __restrict__ dx,
+    W* __restrict__ dw, W* __restrict__ db, float* __restrict__ part) {
+    constexpr int N = kVec<S>, G = bwd_threads(TPR) / TPR;
+    constexpr bool kAhead = TPR < 1024;   // 16 waves a block leave no registers for the next row
+    __shared__ float red[2][bwd_threads(TPR) / 64][2];
+    const int grp = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / TPR));
+    const int i = threadIdx.x % TPR;
+    const Place<N, TPR, kTail> at(i, h);
+    float wv[kChunks][N], aw[kChunks][N], ab[kChunks][N];
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * G;
+    int64_t t = static_cast<int64_t>(blockIdx.x) * G + grp;
+    BwdRow<S> cur, nxt;
+    auto load = [&](BwdRow<S>& row, int64_t at_row) {
+        row.mu = row.r = 0.0f;
+        if (at_row < T) {
+            row.mu = mean[at_row];
+            row.r = rstd[at_row];
+        }
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v) {
+            row.x[v].q = row.dy[v].q = row.res[v].q = Q{0, 0, 0, 0};
+            if (at.on[v] && at_row < T) {
+                const int64_t e = at_row * h + at.off[v];
+                row.dy[v].load(dy + e);
+                row.x[v].load(x + e);
+                if (dres) row.res[v].load(dres + e);
+            }
+        }
+    };
+    load(cur, t);
+#pragma unroll
+    for (int v = 0; v < kChunks; ++v) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            wv[v][j] = 1.0f;
+            aw[v][j] = ab[v][j] = 0.0f;
+        }
+        if (w && at.on[v]) load_params<N>(w + at.off[v], wv[v]);
+    }
+    int turn = 0;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < T; base += stride, t += stride, turn ^= 1) {
+        if constexpr (kAhead) load(nxt, t + stride);
+        float c[2] = {0.0f, 0.0f};   // sums of g xh and of g
+#pragma unroll
+        for (int v = 0; v < kChunks; ++v)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float d = cur.dy[v].at(j), xh = (cur.x[v].at(j) - cur.mu) * cur.r;
+                if constexpr (kSums) {
+                    aw[v][j] += d * xh;
+                    ab[v][j] += d;
+                }
+                const float g = at.counts(v, j) ? d * wv[v][j] : 0.0f;
+                c[0] += g * xh;
+                c[1] += g;
+            }
+        if (dx) {
+            row_sums<2, TPR>(c, red[turn]);
+            const float c1 = c[0] / static_cast<float>(h), c2 = c[1] / static_cast<float>(h);
+            if (t < T) {
+#pragma unroll
+                for (int v = 0; v < kChunks; ++v)
+                    if (at.on[v]) {
+                        float o[N];
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            const float xh = (cur.x[v].at(j) - cur.mu) * cur.r;
+                            o[j] = cur.r * (cur.dy[v].at(j) * wv[v][j] - c2 - xh * c1);
+                            if (dres) o[j] += cur.res[v].at(j);
+                        }
+                        store_chunk(dx + t * h + at.off[v], o);
+                    }
+            }
+        }
+        if constexpr (kAhead)
+            cur = nxt;
+        else
+            load(cur, t + stride);
+    }
+    if constexpr (kSums) {
+        // The block's rows: the groups' sums one after the other, then a partial row each of dw and db (or
+        // the result itself, if this block had all rows).
+        if constexpr (G > 1) {
+            __shared__ float sums[2 * kChunks * N * TPR];
+            for (int g = 1; g < G; ++g) {
+                __syncthreads();
+                if (grp == g) {
+#pragma unroll
+                    for (int v = 0; v < kChunks; ++v)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            sums[(v * N + j) * TPR + i] = aw[v][j];
+                            sums[((kChunks + v) * N + j) * TPR + i] = ab[v][j];
+                        }
+                }
+                __syncthreads();
+                if (grp == 0) {
+#pragma unroll
+                    for (int v = 0; v < kChunks; ++v)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            aw[v][j] += sums[(v * N + j) * TPR + i];
+                            ab[v][j] += sums[((kChunks + v) * N + j) * TPR + i];
+                        }
+                }
+            }
+        }
+        if (grp == 0) {
+            float* p = part + static_cast<int64_t>(blockIdx.x) * 2 * h;
+#pragma unroll
+            for (int v = 0; v < kChunks; ++v)
+                if (at.on[v]) {
+                    if (gridDim.x == 1) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            if (dw) Elem<W>::st(dw, at.off[v] + j, aw[v][j]);
+                            if (db) Elem<W>::st(db, at.off[v] + j, ab[v][j]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < N; k += 4) {
+                            store_chunk(p + at.off[v] + k, aw[v] + k);
+                            store_chunk(p + h + at.off[v] + k, ab[v] + k);
+                        }
+                    }
+                }
+        }
+    }
 }
 
 constexpr int kNormMaxSlices = 256;
@@ -180,13 +499,50 @@ int check_norm(const char* what, int dtype, int w_dtype, int64_t T, int h) {
     return 0;
 }
 
+// Threads a row of the register kernels, or 0: rows shorter than a chunk, longer than 2048 chunks, float64.
+// By h and the type alone, so that a row's bits do not depend on the batch it is in.
+inline int row_threads(int dtype, int h) {
+    if (dtype == RHP_F64) return 0;
+    const int n = 16 / static_cast<int>(dtype_bytes(dtype));
+    if (h < n || h > 2048 * n) return 0;
+    int tpr = 64;
+    while (tpr * kChunks * n < h) tpr *= 2;
+    return tpr;
+}
+
 template <class S, class W>
 int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, double eps, void* y, void* mean,
              void* rstd, hipStream_t stream) {
     using A = typename Elem<S>::acc;
-    hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream,
-                       static_cast<const S*>(x), static_cast<const W*>(w), static_cast<const W*>(b), T, h,
-                       static_cast<A>(eps), static_cast<S*>(y), static_cast<A*>(mean), static_cast<A*>(rstd));
+    const S* xp = static_cast<const S*>(x);
+    const W *wp = static_cast<const W*>(w), *bp = static_cast<const W*>(b);
+    S* yp = static_cast<S*>(y);
+    A *mp = static_cast<A*>(mean), *rp = static_cast<A*>(rstd);
+    if constexpr (sizeof(S) < 8) {
+        const bool tail = h % kVec<S> != 0;
+        auto launch = [&](auto tpr) {
+            constexpr int TPR = decltype(tpr)::value, B = fwd_threads(TPR), G = B / TPR;
+            const dim3 grid(static_cast<unsigned>(
+                std::min<int64_t>((T + G - 1) / G, int64_t(device_cus()) * kFwdBlocksPerCu * 256 / B)));
+            if (tail)
+                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
+                                   static_cast<float>(eps), yp, mp, rp);
+            else
+                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, false>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
+                                   static_cast<float>(eps), yp, mp, rp);
+            return check_launch("norm_fwd_reg_kernel");
+        };
+        switch (row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) {
+            case 64: return launch(std::integral_constant<int, 64>());
+            case 128: return launch(std::integral_constant<int, 128>());
+            case 256: return launch(std::integral_constant<int, 256>());
+            case 512: return launch(std::integral_constant<int, 512>());
+            case 1024: return launch(std::integral_constant<int, 1024>());
+            default: break;
+        }
+    }
+    hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp, wp, bp, T, h,
+                       static_cast<A>(eps), yp, mp, rp);
     return check_launch("norm_fwd_kernel");
 }
 
@@ -194,24 +550,54 @@ template <class S, class W>
 int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, const void* rstd, const void* dres,
              int64_t T, int h, void* dx, void* dw, void* db, void* ws, hipStream_t stream) {
     using A = typename Elem<S>::acc;
-    const S *dyp = static_cast<const S*>(dy), *xp = static_cast<const S*>(x);
+    const S *dyp = static_cast<const S*>(dy), *xp = static_cast<const S*>(x), *resp = static_cast<const S*>(dres);
+    const W* wp = static_cast<const W*>(w);
     const A *mp = static_cast<const A*>(mean), *rp = static_cast<const A*>(rstd);
-    if (dx && T > 0) {
-        hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp,
-                           static_cast<const W*>(w), mp, rp, static_cast<const S*>(dres), T, h, static_cast<S*>(dx));
+    S* dxp = static_cast<S*>(dx);
+    W *dwp = static_cast<W*>(dw), *dbp = static_cast<W*>(db);
+    A* part = static_cast<A*>(ws);
+    const bool sums = dw || db;
+    auto reduce = [&](int parts) {
+        hipLaunchKernelGGL((norm_bwd_reduce_kernel<A, W>), dim3((2 * static_cast<int64_t>(h) + 63) / 64),
+                           dim3(kReduceThreads), 0, stream, part, parts, h, dwp, dbp);
+        return check_launch("norm_bwd_reduce_kernel");
+    };
+    if (T == 0) return sums ? reduce(0) : 0;
+    if constexpr (sizeof(S) < 8) {
+        const bool tail = h % kVec<S> != 0;
+        auto launch = [&](auto tpr) {
+            constexpr int TPR = decltype(tpr)::value, B = bwd_threads(TPR), G = B / TPR;
+            const int64_t nb = std::min<int64_t>((T + G - 1) / G, kNormMaxParts);
+            auto go = [&](auto tl, auto sm) {
+                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value, decltype(sm)::value>),
+                                   dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h,
+                                   dxp, dwp, dbp, part);
+                return check_launch("norm_bwd_reg_kernel");
+            };
+            const int rc = sums ? (tail ? go(std::true_type(), std::true_type()) : go(std::false_type(), std::true_type()))
+                                : (tail ? go(std::true_type(), std::false_type()) : go(std::false_type(), std::false_type()));
+            return rc || !sums || nb == 1 ? rc : reduce(static_cast<int>(nb));
+        };
+        switch (row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) {
+            case 64: return launch(std::integral_constant<int, 64>());
+            case 128: return launch(std::integral_constant<int, 128>());
+            case 256: return launch(std::integral_constant<int, 256>());
+            case 512: return launch(std::integral_constant<int, 512>());
+            case 1024: return launch(std::integral_constant<int, 1024>());
+            default: break;
+        }
+    }
+    if (dx) {
+        hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp, mp,
+                           rp, resp, T, h, dxp);
         if (int rc = check_launch("norm_bwd_rows_kernel")) return rc;
     }
-    if (dw || db) {
-        const int slices = norm_slices(T, h);
-        A* part = static_cast<A*>(ws);
-        hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3((h + 63) / 64, slices), dim3(kNormThreads), 0, stream, dyp,
-                           xp, mp, rp, T, h, slices, part);
-        if (int rc = check_launch("norm_bwd_cols_kernel")) return rc;
-        hipLaunchKernelGGL((norm_bwd_reduce_kernel<A, W>), dim3((2 * h + kNormThreads - 1) / kNormThreads),
-                           dim3(kNormThreads), 0, stream, part, slices, h, static_cast<W*>(dw), static_cast<W*>(db));
-        if (int rc = check_launch("norm_bwd_reduce_kernel")) return rc;
-    }
-    return 0;
+    if (!sums) return 0;
+    const int slices = norm_slices(T, h);
+    hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3((h + 63) / 64, slices), dim3(kNormThreads), 0, stream, dyp, xp, mp,
+                       rp, T, h, slices, part);
+    if (int rc = check_launch("norm_bwd_cols_kernel")) return rc;
+    return reduce(slices);
 }
 
 }  // namespace
@@ -237,7 +623,9 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
 
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
     if (T < 0 || h <= 0) return 0;
-    return static_cast<size_t>(norm_slices(T, h)) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
+    const int64_t parts = row_threads(dtype, h) ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
+                                                : norm_slices(T, h);
+    return static_cast<size_t>(parts) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
 }
 
 extern "C" int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, const void* w, int w_dtype,
