@@ -15,6 +15,12 @@ BLOCK = 128
 M32 = 0xFFFFFFFF
 
 
+def _fma(a, b, c):
+    """a b + c rounded once.  Exact for float32 in float64 but for a second rounding that one value in 2^29 could
+    see; in float64, the mathematics' own type here, the extra rounding does not matter."""
+    return (np.asarray(a, np.float64) * np.asarray(b, np.float64) + np.asarray(c, np.float64)).astype(np.asarray(c).dtype)
+
+
 def update(p, g, m, v, dtype, lr, betas, eps, weight_decay, step, scale=1.0, decay=True):
     """New (p, m, v) as arrays of ``dtype``; ``scale`` multiplies the gradient."""
     t = np.dtype(dtype).type
@@ -23,8 +29,8 @@ def update(p, g, m, v, dtype, lr, betas, eps, weight_decay, step, scale=1.0, dec
     g, m, v = (np.asarray(x).astype(dtype) for x in (g, m, v))
     with np.errstate(all="ignore"):
         g = g * t(scale)
-        m = m * t(b1) + g * c1
-        v = v * t(b2) + (g * c2) * g
+        m = _fma(g, c1, m * t(b1))
+        v = _fma(g * c2, g, v * t(b2))
     return weight(p, m, v, dtype, lr, betas, eps, weight_decay, step, decay), m, v
 
 
@@ -77,8 +83,8 @@ def encode(m: np.ndarray, v: np.ndarray, r: np.ndarray):
     em, ev = _exponent(mag_m), _exponent(mag_v)
     rm, rv = _blocks(r & 0xFFFF), _blocks(r >> 16)
     cm = np.maximum(((mag_m + (rm << 4)) >> 20) - 8 * np.maximum(em - 15, 0)[:, None], 0)
+    cm |= _blocks(bm >> 31) << 7
     with np.errstate(invalid="ignore"):
-        cm |= np.where(_blocks((m < 0).astype(np.int64)) > 0, 128, 0)
         pos = _blocks((v > 0).astype(np.int64)) > 0
     cv = np.maximum(((mag_v + (rv << 4)) >> 20) - 8 * np.maximum(ev - 31, 0)[:, None], 1)
     cv = np.where(pos, cv, 0)

@@ -185,10 +185,16 @@ __device__ __forceinline__ uint32_t random_of(uint32_t x, uint32_t e) {
     return x ^ (x >> 15);
 }
 
-__device__ __forceinline__ uint32_t max16(uint32_t v) {   // over the 16 lanes of a row
-#pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d, 64)));
-    return v;
+// Maximum over the 16 lanes of a DPP row, in all of them: neighbours, pairs, mirrored eights and sixteens.
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    const auto of = [&](auto ctrl) {
+        return static_cast<uint32_t>(
+            __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v = max(v, of(std::integral_constant<int, 0xB1>()));    // quad_perm [1,0,3,2]
+    v = max(v, of(std::integral_constant<int, 0x4E>()));    // quad_perm [2,3,0,1]
+    v = max(v, of(std::integral_constant<int, 0x141>()));   // row_half_mirror
+    return max(v, of(std::integral_constant<int, 0x140>()));   // row_mirror
 }
 // The exponent of a block whose largest magnitude has the bits `top`, such
 // that a magnitude rounded up still has that exponent.
@@ -196,26 +202,23 @@ __device__ __forceinline__ uint32_t exponent_of(uint32_t top) { return min((top 
 __device__ __forceinline__ int base_of(uint32_t e, int binades) {
     return max(static_cast<int>(e) - (binades - 1), 0) * 8;
 }
-__device__ __forceinline__ float decode_m(uint32_t q, uint32_t e) {
-    if (e == 255) return __builtin_nanf("");
+// base = base_of(the block's exponent); the exponent 255 is the caller's to see.
+__device__ __forceinline__ float decode_m(uint32_t q, int base) {
     const uint32_t c = q & 127;
-    const uint32_t bits = ((c + static_cast<uint32_t>(base_of(e, 16))) << 20) | ((q & 128) << 24);
+    const uint32_t bits = ((c + static_cast<uint32_t>(base)) << 20) | ((q << 24) & 0x80000000u);
     return c ? __uint_as_float(bits) : 0.0f;
 }
-__device__ __forceinline__ float decode_v(uint32_t q, uint32_t e) {
-    if (e == 255) return __builtin_nanf("");
-    return q ? __uint_as_float((q + static_cast<uint32_t>(base_of(e, 32))) << 20) : 0.0f;
+__device__ __forceinline__ float decode_v(uint32_t q, int base) {
+    return q ? __uint_as_float((q + static_cast<uint32_t>(base)) << 20) : 0.0f;
 }
-__device__ __forceinline__ uint32_t encode_m(float m, uint32_t e, uint32_t r) {
-    if (e == 255) return 0;
-    const uint32_t b = __float_as_uint(m);
-    const int c = static_cast<int>(((b & 0x7FFFFFFFu) + ((r & 0xFFFFu) << 4)) >> 20) - base_of(e, 16);
-    return static_cast<uint32_t>(max(c, 0)) | (m < 0.0f ? 128u : 0u);
+// bits: of the moment; r: the 16 random bits.  v is 0 only for 0: min(.., bits) is 0 there and nowhere else.
+__device__ __forceinline__ uint32_t encode_m(uint32_t bits, int base, uint32_t r) {
+    const int c = static_cast<int>((bits & 0x7FFFFFFFu) + (r << 4) - (static_cast<uint32_t>(base) << 20)) >> 20;
+    return static_cast<uint32_t>(max(c, 0)) | ((bits >> 24) & 128u);
 }
-__device__ __forceinline__ uint32_t encode_v(float v, uint32_t e, uint32_t r) {
-    if (e == 255 || !(v > 0.0f)) return 0;
-    const int c = static_cast<int>((__float_as_uint(v) + ((r >> 16) << 4)) >> 20) - base_of(e, 32);
-    return static_cast<uint32_t>(max(c, 1));
+__device__ __forceinline__ uint32_t encode_v(uint32_t bits, int base, uint32_t r) {
+    const int c = static_cast<int>(bits + (r << 4) - (static_cast<uint32_t>(base) << 20)) >> 20;
+    return min(static_cast<uint32_t>(max(c, 1)), bits);
 }
 
 // Eight codes at p + e (those at n and past it read as 0 and are not stored).
@@ -253,24 +256,50 @@ __device__ __forceinline__ void store_scales(uint8_t* p, int64_t e, uint32_t em,
     *(RHP_GLOBAL H*)(reinterpret_cast<uintptr_t>(p + e / kScaleBlock * 2)) = static_cast<uint16_t>(em | ev << 8);
 }
 
-// Encodes eight elements a lane, 16 lanes a block of 128, and stores the
-// block's exponents.  Every lane of the wave takes part; a lane past the
-// tensor's end brings zeros.
-__device__ __forceinline__ void encode_group(const float* m, const float* v, uint32_t hash, int64_t e0, int64_t n,
+// Eight elements' values from their codes; every one of a block that is not finite is NaN.
+__device__ __forceinline__ void decode_group(const uint32_t* cm, const uint32_t* cv, uint32_t em, uint32_t ev,
+                                             float* m, float* v) {
+    const int bm = base_of(em, 16), bv = base_of(ev, 32);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = decode_m(cm[i], bm);
+        v[i] = decode_v(cv[i], bv);
+    }
+    if (em == 255 || ev == 255) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (em == 255) m[i] = __builtin_nanf("");
+            if (ev == 255) v[i] = __builtin_nanf("");
+        }
+    }
+}
+
+// Encodes eight elements a lane, 16 lanes a block of 128, with the random bits random(i), and stores them with
+// the block's exponents.  Every lane of the wave takes part; a lane past the tensor's end brings zeros.
+template <class Random>
+__device__ __forceinline__ void encode_group(const float* m, const float* v, Random random, int64_t e0, int64_t n,
                                              uint8_t* qm, uint8_t* qv, uint8_t* scales) {
     uint32_t tm = 0, tv = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         tm = max(tm, __float_as_uint(m[i]) & 0x7FFFFFFFu);
-        tv = max(tv, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        tv = max(tv, __float_as_uint(v[i]));   // a v with a sign is a NaN
     }
-    const uint32_t em = exponent_of(max16(tm)), ev = exponent_of(max16(tv));
+    const uint32_t em = exponent_of(max16(tm)), ev = exponent_of(max16(tv) & 0x7FFFFFFFu);
+    const int bm = base_of(em, 16), bv = base_of(ev, 32);
     uint32_t cm[8], cv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t r = random_of(hash, i);
-        cm[i] = encode_m(m[i], em, r);
-        cv[i] = encode_v(v[i], ev, r);
+        const uint32_t r = random(i);
+        cm[i] = encode_m(__float_as_uint(m[i]), bm, r & 0xFFFFu);
+        cv[i] = encode_v(__float_as_uint(v[i]), bv, r >> 16);
+    }
+    if (em == 255 || ev == 255) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (em == 255) cm[i] = 0;
+            if (ev == 255) cv[i] = 0;
+        }
     }
     if (e0 < n) {
         store_codes(qm, e0, n, cm);
@@ -290,17 +319,35 @@ struct Grads {
 };
 constexpr int kDtypeShift = 60;
 
-__device__ __forceinline__ float sqrt_of(float x) { return __builtin_sqrtf(x); }
-__device__ __forceinline__ double sqrt_of(double x) { return __builtin_sqrt(x); }
+// sqrt(v) and m / d.  In float by the hardware's square root and reciprocal (each within one unit in the last
+// place; the update is rounded once more into a weight some hundred times its size).  They may take subnormals
+// for zero: a subnormal v has a root under 1.1e-19, which beside eps >= 2e-12 is less than half a unit of d.
+// With a smaller eps (kTinyEps) the correctly rounded forms run.
+template <bool kTinyEps> __device__ __forceinline__ float sqrt_of(float x) {
+    return kTinyEps ? __builtin_sqrtf(x) : __builtin_amdgcn_sqrtf(x);
+}
+template <bool kTinyEps> __device__ __forceinline__ double sqrt_of(double x) { return __builtin_sqrt(x); }
+template <bool kTinyEps> __device__ __forceinline__ float quotient(float m, float d) {
+    return kTinyEps ? m / d : m * __builtin_amdgcn_rcpf(d);
+}
+template <bool kTinyEps> __device__ __forceinline__ double quotient(double m, double d) { return m / d; }
+constexpr double kLeastFastEps = 2e-12;
+__device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_of(double a, double b, double c) { return a * b + c; }
 
-template <int N, class A> __device__ __forceinline__ void update(const Scalars<A>& s, A keep, A gs, A* p, const A* g, A* m, A* v) {
+template <int N, bool kTinyEps, class A>
+__device__ __forceinline__ void update(const Scalars<A>& s, A keep, const float* grad_scale, A* p, A* g, A* m, A* v) {
+    if (grad_scale) {
+        const A gs = static_cast<A>(*grad_scale);
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= gs;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const A x = g[i] * gs;
-        m[i] = m[i] * s.b1 + x * s.c1;
-        v[i] = v[i] * s.b2 + (x * s.c2) * x;
-        const A d = sqrt_of(v[i]) * s.ibc2s + s.eps;
-        p[i] = p[i] * keep - s.a * (m[i] / d);
+        m[i] = fma_of(g[i], s.c1, m[i] * s.b1);
+        v[i] = fma_of(g[i] * s.c2, g[i], v[i] * s.b2);
+        const A d = fma_of(sqrt_of<kTinyEps>(v[i]), s.ibc2s, s.eps);
+        p[i] = fma_of(-s.a, quotient<kTinyEps>(m[i], d), p[i] * keep);
     }
 }
 
@@ -346,58 +393,57 @@ template <int N, class A> __device__ __forceinline__ void store_weight(const Pla
     }
 }
 
-template <class A, bool kState8>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const uint8_t* __restrict__ plan, Grads grads, uint32_t t0,
-                                                         uint32_t b0, Scalars<A> s, const float* __restrict__ grad_scale,
-                                                         uint32_t salt) {
-    const PlanHeader& head = *reinterpret_cast<const PlanHeader*>(plan);
-    const PlanTensor* tensors = reinterpret_cast<const PlanTensor*>(plan + sizeof(PlanHeader));
-    const uint32_t* of_block = reinterpret_cast<const uint32_t*>(tensors + head.count);
+template <class A, bool kState8, bool kTinyEps>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const PlanTensor* __restrict__ tensors,
+                                                         const uint32_t* __restrict__ of_block, Grads grads,
+                                                         uint32_t t0, uint32_t b0, Scalars<A> s,
+                                                         const float* __restrict__ grad_scale, uint32_t salt) {
     const uint32_t b = b0 + blockIdx.x;
     const uint32_t ti = of_block[b];
     const PlanTensor t = tensors[ti];
     const uint64_t g = grads.g[ti - t0];
-    const A gs = grad_scale ? static_cast<A>(*grad_scale) : A(1);
     const A keep = t.decay ? s.keep : A(1);
     const int64_t base = static_cast<int64_t>(b - t.block0) * kBlockElems;
     if constexpr (kState8) {
         const int64_t e0 = base + threadIdx.x * 8;
-        uint32_t cm[8], cv[8];
+        uint32_t cm[8], cv[8], em = 0, ev = 0;
         float p[8], gv[8], m[8], v[8];
         load_codes(static_cast<const uint8_t*>(t.m), e0, t.n, cm);
         load_codes(static_cast<const uint8_t*>(t.v), e0, t.n, cv);
+        if (e0 < t.n) load_scales(t.scales, e0, &em, &ev);
         load_weight<8>(t, e0, p);
         load_grad<8>(g, e0, t.n, gv);
-        const bool in = e0 < t.n;
-        uint32_t em = 0, ev = 0;
-        if (in) load_scales(t.scales, e0, &em, &ev);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = in ? decode_m(cm[i], em) : 0.0f;
-            v[i] = in ? decode_v(cv[i], ev) : 0.0f;
-        }
-        update<8>(s, keep, gs, p, gv, m, v);
+        decode_group(cm, cv, em, ev, m, v);
+        update<8, kTinyEps>(s, keep, grad_scale, p, gv, m, v);
         store_weight<8>(t, e0, p);
-        // Elements past the end read as zeros and, but in a block that is not finite, stay zeros.
+        if (e0 + 8 > t.n) {
+            // Elements past the end read as zeros and, but in a block that is not finite, stay zeros.
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (e0 + i >= t.n) m[i] = v[i] = 0.0f;
+            for (int i = 0; i < 8; ++i)
+                if (e0 + i >= t.n) m[i] = v[i] = 0.0f;
+        }
         const uint32_t hash = mix(mix(t.key ^ salt) + static_cast<uint32_t>(e0 >> 3));
-        encode_group(m, v, hash, e0, t.n, static_cast<uint8_t*>(t.m), static_cast<uint8_t*>(t.v), t.scales);
+        encode_group(m, v, [&](int i) { return random_of(hash, i); }, e0, t.n, static_cast<uint8_t*>(t.m),
+                     static_cast<uint8_t*>(t.v), t.scales);
     } else {
+        // All loads of a thread's two groups before the first update: a store could alias a later load.
+        constexpr int U = 2;
+        A p[U][4], gv[U][4], m[U][4], v[U][4];
+        int64_t e0[U];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int64_t e0 = base + u * (kBlockElems / 2) + threadIdx.x * 4;
-            if (e0 >= t.n) return;
-            A p[4], gv[4], m[4], v[4];
-            load_n<4>(static_cast<const A*>(t.m), e0, t.n, m);
-            load_n<4>(static_cast<const A*>(t.v), e0, t.n, v);
-            load_weight<4>(t, e0, p);
-            load_grad<4>(g, e0, t.n, gv);
-            update<4>(s, keep, gs, p, gv, m, v);
-            store_weight<4>(t, e0, p);
-            store_n<4>(static_cast<A*>(t.m), e0, t.n, m);
-            store_n<4>(static_cast<A*>(t.v), e0, t.n, v);
+        for (int u = 0; u < U; ++u) {
+            e0[u] = base + u * (kBlockElems / U) + threadIdx.x * 4;
+            load_n<4>(static_cast<const A*>(t.m), e0[u], t.n, m[u]);
+            load_n<4>(static_cast<const A*>(t.v), e0[u], t.n, v[u]);
+            load_weight<4>(t, e0[u], p[u]);
+            load_grad<4>(g, e0[u], t.n, gv[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            update<4, kTinyEps>(s, keep, grad_scale, p[u], gv[u], m[u], v[u]);
+            store_weight<4>(t, e0[u], p[u]);
+            store_n<4>(static_cast<A*>(t.m), e0[u], t.n, m[u]);
+            store_n<4>(static_cast<A*>(t.v), e0[u], t.n, v[u]);
         }
     }
 }
@@ -415,11 +461,7 @@ __global__ __launch_bounds__(kThreads) void moments_decode_kernel(const uint8_t*
     load_codes(qv, e0, n, cv);
     uint32_t em, ev;
     load_scales(scales, e0, &em, &ev);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        a[i] = decode_m(cm[i], em);
-        b[i] = decode_v(cv[i], ev);
-    }
+    decode_group(cm, cv, em, ev, a, b);
     store_n<8>(m, e0, n, a);
     store_n<8>(v, e0, n, b);
 }
@@ -431,23 +473,7 @@ __global__ __launch_bounds__(kThreads) void moments_encode_kernel(const float* _
     float a[8], b[8];
     load_n<8>(m, e0, n, a);
     load_n<8>(v, e0, n, b);
-    uint32_t tm = 0, tv = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        tm = max(tm, __float_as_uint(a[i]) & 0x7FFFFFFFu);
-        tv = max(tv, __float_as_uint(b[i]) & 0x7FFFFFFFu);
-    }
-    const uint32_t em = exponent_of(max16(tm)), ev = exponent_of(max16(tv));
-    uint32_t cm[8], cv[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        cm[i] = encode_m(a[i], em, 0x80008000u);
-        cv[i] = encode_v(b[i], ev, 0x80008000u);
-    }
-    if (e0 >= n) return;
-    store_codes(qm, e0, n, cm);
-    store_codes(qv, e0, n, cv);
-    if ((threadIdx.x & 15) == 0) store_scales(scales, e0, em, ev);
+    encode_group(a, b, [](int) { return 0x80008000u; }, e0, n, qm, qv, scales);
 }
 
 // ------------------------------------------------------------------ the gradients' norm
@@ -537,11 +563,13 @@ inline uint64_t tag(const void* p, int dt) {
     return reinterpret_cast<uint64_t>(p) | static_cast<uint64_t>(dt) << kDtypeShift;
 }
 
-template <class A, bool kState8>
+template <class A, bool kState8, bool kTinyEps>
 int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grads, const int* g_dtypes,
                 const Scalars<A>& s, const float* grad_scale, uint32_t salt, hipStream_t stream) {
     const PlanHeader& head = *reinterpret_cast<const PlanHeader*>(host);
     const PlanTensor* ts = reinterpret_cast<const PlanTensor*>(host + sizeof(PlanHeader));
+    const PlanTensor* tensors = reinterpret_cast<const PlanTensor*>(dev + sizeof(PlanHeader));
+    const uint32_t* of_block = reinterpret_cast<const uint32_t*>(tensors + head.count);
     for (uint32_t t0 = 0; t0 < head.count; t0 += kMaxGrads) {
         const uint32_t t1 = std::min(head.count, t0 + kMaxGrads);
         const uint32_t b0 = ts[t0].block0, b1 = t1 < head.count ? ts[t1].block0 : head.blocks;
@@ -549,8 +577,8 @@ int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grad
         Grads g{};
         for (uint32_t t = t0; t < t1; ++t)
             if (grads && grads[t]) g.g[t - t0] = tag(grads[t], g_dtypes[t]);
-        hipLaunchKernelGGL((adamw_kernel<A, kState8>), dim3(b1 - b0), dim3(kThreads), 0, stream, dev, g, t0, b0, s,
-                           grad_scale, salt);
+        hipLaunchKernelGGL((adamw_kernel<A, kState8, kTinyEps>), dim3(b1 - b0), dim3(kThreads), 0, stream, tensors,
+                           of_block, g, t0, b0, s, grad_scale, salt);
         if (int rc = check_launch("adamw_kernel")) return rc;
     }
     return 0;
@@ -648,12 +676,16 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
                                   static_cast<uint32_t>(seed >> 32)) ^
                               static_cast<uint32_t>(seed));
     const uint8_t* dev = static_cast<const uint8_t*>(dev_image);
-    if (head.f64) return launch_step<double, false>(host, dev, grads, g_dtypes, d, grad_scale, salt, stream);
+    const auto go = [&](auto launch, const auto& scalars) {
+        return launch(host, dev, grads, g_dtypes, scalars, grad_scale, salt, stream);
+    };
+    if (head.f64) return go(launch_step<double, false, false>, d);
     const Scalars<float> f{static_cast<float>(d.b1), static_cast<float>(d.c1), static_cast<float>(d.b2),
                            static_cast<float>(d.c2), static_cast<float>(d.ibc2s), static_cast<float>(d.eps),
                            static_cast<float>(d.a), static_cast<float>(d.keep)};
-    if (head.state8) return launch_step<float, true>(host, dev, grads, g_dtypes, f, grad_scale, salt, stream);
-    return launch_step<float, false>(host, dev, grads, g_dtypes, f, grad_scale, salt, stream);
+    if (eps < kLeastFastEps)
+        return head.state8 ? go(launch_step<float, true, true>, f) : go(launch_step<float, false, true>, f);
+    return head.state8 ? go(launch_step<float, true, false>, f) : go(launch_step<float, false, false>, f);
 }
 
 static int check_codes(const char* what, int64_t n, const void* const* ptrs, int count) {
