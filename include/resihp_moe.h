@@ -488,7 +488,7 @@ int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, const void* w, 
  * index): the same arguments give the same codes.  v > 0 never becomes 0.
  * E = 255 marks a block with a value that is not finite: it reads as NaN.
  */
-size_t rhp_adamw_plan_bytes(int count, const int64_t* numel);
+size_t rhp_adamw_plan_bytes(int count, const int64_t* numel, int state_bits);
 int rhp_adamw_plan(int count, void* const* params, const int* dtypes, void* const* masters, void* const* exp_avg,
                    void* const* exp_avg_sq, void* const* scales, const int64_t* numel, const uint32_t* keys,
                    const int* decay, int state_bits, void* image, size_t image_bytes);

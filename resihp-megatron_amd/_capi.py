@@ -62,7 +62,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "rhp_layer_norm_fwd": (_i, [_p, _i, _p, _p, _i, _i64, _i, _d, _p, _p, _p, _p]),
     "rhp_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
     "rhp_layer_norm_bwd": (_i, [_p, _p, _i, _p, _i, _p, _p, _p, _i64, _i, _p, _p, _p, _p, _sz, _p]),
-    "rhp_adamw_plan_bytes": (_sz, [_i, _p]),
+    "rhp_adamw_plan_bytes": (_sz, [_i, _p, _i]),
     "rhp_adamw_plan": (_i, [_i, _pp, _p, _pp, _pp, _pp, _pp, _p, _p, _p, _i, _p, _sz]),
     "rhp_adamw_step": (_i, [_p, _p, _sz, _pp, _p, _d, _d, _d, _d, _d, _i64, _p, _u64, _p]),
     "rhp_moments_decode": (_i, [_p, _p, _p, _i64, _p, _p, _p]),

@@ -42,7 +42,8 @@ namespace rhp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlockElems = 2048;      // elements a block steps
+constexpr int kElems8 = 8, kElems32 = 4;   // elements a thread steps
+constexpr int kBlock8 = kThreads * kElems8, kBlock32 = kThreads * kElems32;
 constexpr int kScaleBlock = 128;       // elements that share an exponent
 constexpr int kMaxGrads = 448;         // tensors a launch takes (their gradients' pointers are kernel arguments)
 
@@ -67,7 +68,10 @@ struct PlanTensor {
 };
 static_assert(sizeof(PlanHeader) == 32 && sizeof(PlanTensor) == 64, "plan layout");
 
-inline int64_t blocks_of(int64_t n) { return (n + kBlockElems - 1) / kBlockElems; }
+inline int64_t blocks_of(int64_t n, bool state8) {
+    const int64_t k = state8 ? kBlock8 : kBlock32;
+    return (n + k - 1) / k;
+}
 inline size_t plan_bytes(uint64_t count, uint64_t blocks) {
     return sizeof(PlanHeader) + count * sizeof(PlanTensor) + blocks * 4;
 }
@@ -403,9 +407,9 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const PlanTensor* __res
     const PlanTensor t = tensors[ti];
     const uint64_t g = grads.g[ti - t0];
     const A keep = t.decay ? s.keep : A(1);
-    const int64_t base = static_cast<int64_t>(b - t.block0) * kBlockElems;
+    const int64_t e0 = static_cast<int64_t>(b - t.block0) * (kState8 ? kBlock8 : kBlock32) +
+                       threadIdx.x * (kState8 ? kElems8 : kElems32);
     if constexpr (kState8) {
-        const int64_t e0 = base + threadIdx.x * 8;
         uint32_t cm[8], cv[8], em = 0, ev = 0;
         float p[8], gv[8], m[8], v[8];
         load_codes(static_cast<const uint8_t*>(t.m), e0, t.n, cm);
@@ -426,25 +430,15 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const PlanTensor* __res
         encode_group(m, v, [&](int i) { return random_of(hash, i); }, e0, t.n, static_cast<uint8_t*>(t.m),
                      static_cast<uint8_t*>(t.v), t.scales);
     } else {
-        // All loads of a thread's two groups before the first update: a store could alias a later load.
-        constexpr int U = 2;
-        A p[U][4], gv[U][4], m[U][4], v[U][4];
-        int64_t e0[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            e0[u] = base + u * (kBlockElems / U) + threadIdx.x * 4;
-            load_n<4>(static_cast<const A*>(t.m), e0[u], t.n, m[u]);
-            load_n<4>(static_cast<const A*>(t.v), e0[u], t.n, v[u]);
-            load_weight<4>(t, e0[u], p[u]);
-            load_grad<4>(g, e0[u], t.n, gv[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            update<4, kTinyEps>(s, keep, grad_scale, p[u], gv[u], m[u], v[u]);
-            store_weight<4>(t, e0[u], p[u]);
-            store_n<4>(static_cast<A*>(t.m), e0[u], t.n, m[u]);
-            store_n<4>(static_cast<A*>(t.v), e0[u], t.n, v[u]);
-        }
+        A p[kElems32], gv[kElems32], m[kElems32], v[kElems32];
+        load_n<kElems32>(static_cast<const A*>(t.m), e0, t.n, m);
+        load_n<kElems32>(static_cast<const A*>(t.v), e0, t.n, v);
+        load_weight<kElems32>(t, e0, p);
+        load_grad<kElems32>(g, e0, t.n, gv);
+        update<kElems32, kTinyEps>(s, keep, grad_scale, p, gv, m, v);
+        store_weight<kElems32>(t, e0, p);
+        store_n<kElems32>(static_cast<A*>(t.m), e0, t.n, m);
+        store_n<kElems32>(static_cast<A*>(t.v), e0, t.n, v);
     }
 }
 
@@ -589,12 +583,12 @@ int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grad
 
 using namespace rhp;
 
-extern "C" size_t rhp_adamw_plan_bytes(int count, const int64_t* numel) {
-    if (count < 0 || (count > 0 && !numel)) return 0;
+extern "C" size_t rhp_adamw_plan_bytes(int count, const int64_t* numel, int state_bits) {
+    if (count < 0 || (count > 0 && !numel) || (state_bits != 32 && state_bits != 8)) return 0;
     uint64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] < 0) return 0;
-        blocks += static_cast<uint64_t>(blocks_of(numel[i]));
+        blocks += static_cast<uint64_t>(blocks_of(numel[i], state_bits == 8));
     }
     return plan_bytes(static_cast<uint64_t>(count), blocks);
 }
@@ -616,7 +610,7 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
         RHP_REQUIRE(float_dtype(dtypes[i]), std::string("rhp_adamw_plan: unsupported dtype ") + dtype_name(dtypes[i]));
         (dtypes[i] == RHP_F64 ? any64 : other) = true;
         RHP_REQUIRE(!masters || !masters[i] || dtypes[i] == RHP_BF16, "rhp_adamw_plan: masters are for bfloat16 weights");
-        blocks += static_cast<uint64_t>(blocks_of(numel[i]));
+        blocks += static_cast<uint64_t>(blocks_of(numel[i], state_bits == 8));
         if (numel[i] == 0) continue;
         RHP_REQUIRE(params[i] && exp_avg[i] && exp_avg_sq[i] && (state_bits == 32 || scales[i]),
                     "rhp_adamw_plan: null tensor");
@@ -642,7 +636,7 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
                            state_bits == 8 ? static_cast<uint8_t*>(scales[i]) : nullptr, numel[i], keys ? keys[i] : 0u,
                            b, static_cast<uint32_t>(dtypes[i]), static_cast<uint32_t>(!decay || decay[i])};
         std::memcpy(&ts[i], &t, sizeof t);
-        for (int64_t k = blocks_of(numel[i]); k > 0; --k) of_block[b++] = static_cast<uint32_t>(i);
+        for (int64_t k = blocks_of(numel[i], state_bits == 8); k > 0; --k) of_block[b++] = static_cast<uint32_t>(i);
     }
     return 0;
 }
@@ -701,7 +695,7 @@ extern "C" int rhp_moments_decode(const uint8_t* q_m, const uint8_t* q_v, const 
     if (int rc = check_codes("rhp_moments_decode", n, ptrs, 5)) return rc;
     if (n == 0) return 0;
     RHP_REQUIRE(element_aligned(m, RHP_BF16) && element_aligned(v, RHP_BF16), "rhp_moments_decode: unaligned output");
-    hipLaunchKernelGGL(moments_decode_kernel, dim3(static_cast<unsigned>((n + kBlockElems - 1) / kBlockElems)),
+    hipLaunchKernelGGL(moments_decode_kernel, dim3(static_cast<unsigned>((n + kBlock8 - 1) / kBlock8)),
                        dim3(kThreads), 0, stream, q_m, q_v, scales, n, static_cast<bf16*>(m), static_cast<bf16*>(v));
     return check_launch("moments_decode_kernel");
 }
@@ -713,7 +707,7 @@ extern "C" int rhp_moments_encode(const float* m, const float* v, int64_t n, uin
     if (int rc = check_codes("rhp_moments_encode", n, ptrs, 5)) return rc;
     if (n == 0) return 0;
     RHP_REQUIRE(element_aligned(m, RHP_F32) && element_aligned(v, RHP_F32), "rhp_moments_encode: unaligned input");
-    hipLaunchKernelGGL(moments_encode_kernel, dim3(static_cast<unsigned>((n + kBlockElems - 1) / kBlockElems)),
+    hipLaunchKernelGGL(moments_encode_kernel, dim3(static_cast<unsigned>((n + kBlock8 - 1) / kBlock8)),
                        dim3(kThreads), 0, stream, m, v, n, q_m, q_v, scales);
     return check_launch("moments_encode_kernel");
 }

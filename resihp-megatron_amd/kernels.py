@@ -859,7 +859,7 @@ class AdamWPlan:
         self.dtypes = [p.dtype for p in params]
         self.ptrs = [p.data_ptr() for p in params]
         numel = _int_array(ctypes.c_int64, [p.numel() for p in params])
-        size = C.lib().rhp_adamw_plan_bytes(n, numel)
+        size = C.lib().rhp_adamw_plan_bytes(n, numel, 8 if eight else 32)
         self.image = torch.empty(size, dtype=torch.uint8)
         addr = lambda ts: C.ptr_array([0 if t is None else t.data_ptr() for t in ts])  # noqa: E731
         C.call("rhp_adamw_plan", n, addr(params), _int_array(ctypes.c_int, [_DT[p.dtype] for p in params]),

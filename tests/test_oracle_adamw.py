@@ -106,7 +106,7 @@ def _plan(numel=(10,), dtypes=(C.BF16,), params=(FAKE,), m=(FAKE,), v=(FAKE,), s
           bits=32, short=0):
     n = len(numel)
     num = (ctypes.c_int64 * n)(*numel)
-    size = C.lib().rhp_adamw_plan_bytes(n, num)
+    size = C.lib().rhp_adamw_plan_bytes(n, num, bits)
     buf = ctypes.create_string_buffer(max(1, size))
     C.call("rhp_adamw_plan", n, C.ptr_array(params), (ctypes.c_int * n)(*dtypes), C.ptr_array(masters) if masters else None,
            C.ptr_array(m), C.ptr_array(v), C.ptr_array(scales) if scales else None, num,
@@ -135,7 +135,8 @@ def test_plan_refusals(kw, msg):
 
 def test_plan_refuses_bad_counts():
     num = (ctypes.c_int64 * 1)(-1)
-    assert C.lib().rhp_adamw_plan_bytes(1, num) == 0 and C.lib().rhp_adamw_plan_bytes(-1, None) == 0
+    assert C.lib().rhp_adamw_plan_bytes(1, num, 32) == 0 and C.lib().rhp_adamw_plan_bytes(-1, None, 32) == 0
+    assert C.lib().rhp_adamw_plan_bytes(0, None, 16) == 0 and C.lib().rhp_adamw_plan_bytes(0, None, 8) > 0
     buf = ctypes.create_string_buffer(4096)
     for n in (-1, (1 << 34) + 1):
         with pytest.raises(RuntimeError, match="out of range"):
