@@ -42,7 +42,7 @@ namespace rhp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kElems8 = 8, kElems32 = 4;   // elements a thread steps
+constexpr int kGroups8 = 2, kElems8 = 8 * kGroups8, kElems32 = 4;   // elements a thread steps
 constexpr int kBlock8 = kThreads * kElems8, kBlock32 = kThreads * kElems32;
 constexpr int kScaleBlock = 128;       // elements that share an exponent
 constexpr int kMaxGrads = 448;         // tensors a launch takes (their gradients' pointers are kernel arguments)
@@ -206,44 +206,49 @@ __device__ __forceinline__ uint32_t exponent_of(uint32_t top) { return min((top 
 __device__ __forceinline__ int base_of(uint32_t e, int binades) {
     return max(static_cast<int>(e) - (binades - 1), 0) * 8;
 }
-// base = base_of(the block's exponent); the exponent 255 is the caller's to see.
-__device__ __forceinline__ float decode_m(uint32_t q, int base) {
-    const uint32_t c = q & 127;
-    const uint32_t bits = ((c + static_cast<uint32_t>(base)) << 20) | ((q << 24) & 0x80000000u);
-    return c ? __uint_as_float(bits) : 0.0f;
+// The values of byte k of a word of codes; base = base_of(the block's exponent), whose 255 is the caller's to see.
+__device__ __forceinline__ float decode_m(uint32_t w, int k, int base) {
+    const uint32_t c = (w >> (8 * k)) & 127, sign = (w << (24 - 8 * k)) & 0x80000000u;
+    return c ? __uint_as_float(((c + static_cast<uint32_t>(base)) << 20) | sign) : 0.0f;
 }
-__device__ __forceinline__ float decode_v(uint32_t q, int base) {
-    return q ? __uint_as_float((q + static_cast<uint32_t>(base)) << 20) : 0.0f;
+__device__ __forceinline__ float decode_v(uint32_t w, int k, int base) {
+    const uint32_t c = (w >> (8 * k)) & 255;
+    return c ? __uint_as_float((c + static_cast<uint32_t>(base)) << 20) : 0.0f;
 }
-// bits: of the moment; r: the 16 random bits.  v is 0 only for 0: min(.., bits) is 0 there and nowhere else.
-__device__ __forceinline__ uint32_t encode_m(uint32_t bits, int base, uint32_t r) {
-    const int c = static_cast<int>((bits & 0x7FFFFFFFu) + (r << 4) - (static_cast<uint32_t>(base) << 20)) >> 20;
-    return static_cast<uint32_t>(max(c, 0)) | ((bits >> 24) & 128u);
+// bits: of the moment; r: the 16 random bits.  Without the low four bits of the moment, which no carry leaves,
+// the random bits and the code lie in half-words.
+__device__ __forceinline__ uint32_t encode_m(uint32_t bits, int base, uint32_t r) {   // without the sign
+    return static_cast<uint32_t>(max(static_cast<int>((((bits >> 4) & 0x7FFFFFFu) + r) >> 16) - base, 0));
 }
 __device__ __forceinline__ uint32_t encode_v(uint32_t bits, int base, uint32_t r) {
-    const int c = static_cast<int>(bits + (r << 4) - (static_cast<uint32_t>(base) << 20)) >> 20;
-    return min(static_cast<uint32_t>(max(c, 1)), bits);
+    // At least 1 for what is not 0: the middle of (code, 1, bits), bits being 0 only for 0 and never under a code.
+    const int c = static_cast<int>(((bits >> 4) + r) >> 16) - base, b = static_cast<int>(bits);
+    return static_cast<uint32_t>(max(min(max(c, 1), b), min(c, 1)));
+}
+// Four bytes from the low (kByte 0) or high (3) bytes of four words.
+template <int kByte> __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    constexpr uint32_t kPair = (uint32_t(kByte) + 4) << 8 | uint32_t(kByte);       // byte of the 2nd and of the 1st operand
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0000u | kPair);
+    const uint32_t hi = __builtin_amdgcn_perm(d, c, kPair << 16 | 0x00000C0Cu);
+    return lo | hi;
 }
 
 // Eight codes at p + e (those at n and past it read as 0 and are not stored).
-__device__ __forceinline__ void load_codes(const uint8_t* p, int64_t e, int64_t n, uint32_t* q) {
-    if (e + 8 <= n) {
-        const U2 t = load_at<U2a>(p + e);
+__device__ __forceinline__ U2 load_codes(const uint8_t* p, int64_t e, int64_t n) {
+    if (e + 8 <= n) return load_at<U2a>(p + e);
+    U2 q = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (t[i / 4] >> (8 * (i & 3))) & 255;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = e + i < n ? load_at<uint8_t>(p + e + i) : 0;
-    }
+    for (int i = 0; i < 8; ++i)
+        if (e + i < n) q[i / 4] |= static_cast<uint32_t>(load_at<uint8_t>(p + e + i)) << (8 * (i & 3));
+    return q;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int64_t n, const uint32_t* q) {
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int64_t n, U2 q) {
     if (e + 8 <= n) {
-        const U2 t = {q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
-        store_at<U2a>(p + e, t);
+        store_at<U2a>(p + e, q);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (e + i < n) store_at<uint8_t>(p + e + i, static_cast<uint8_t>(q[i]));
+            if (e + i < n) store_at<uint8_t>(p + e + i, static_cast<uint8_t>(q[i / 4] >> (8 * (i & 3))));
     }
 }
 
@@ -261,13 +266,12 @@ __device__ __forceinline__ void store_scales(uint8_t* p, int64_t e, uint32_t em,
 }
 
 // Eight elements' values from their codes; every one of a block that is not finite is NaN.
-__device__ __forceinline__ void decode_group(const uint32_t* cm, const uint32_t* cv, uint32_t em, uint32_t ev,
-                                             float* m, float* v) {
+__device__ __forceinline__ void decode_group(U2 qm, U2 qv, uint32_t em, uint32_t ev, float* m, float* v) {
     const int bm = base_of(em, 16), bv = base_of(ev, 32);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        m[i] = decode_m(cm[i], bm);
-        v[i] = decode_v(cv[i], bv);
+        m[i] = decode_m(qm[i / 4], i & 3, bm);
+        v[i] = decode_v(qv[i / 4], i & 3, bv);
     }
     if (em == 255 || ev == 255) {
 #pragma unroll
@@ -291,23 +295,29 @@ __device__ __forceinline__ void encode_group(const float* m, const float* v, Ran
     }
     const uint32_t em = exponent_of(max16(tm)), ev = exponent_of(max16(tv) & 0x7FFFFFFFu);
     const int bm = base_of(em, 16), bv = base_of(ev, 32);
-    uint32_t cm[8], cv[8];
+    uint32_t cm[8], cv[8], bits[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t r = random(i);
-        cm[i] = encode_m(__float_as_uint(m[i]), bm, r & 0xFFFFu);
+        bits[i] = __float_as_uint(m[i]);
+        cm[i] = encode_m(bits[i], bm, r & 0xFFFFu);
         cv[i] = encode_v(__float_as_uint(v[i]), bv, r >> 16);
     }
-    if (em == 255 || ev == 255) {
+    U2 pm, pv;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (em == 255) cm[i] = 0;
-            if (ev == 255) cv[i] = 0;
-        }
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t* c = cm + 4 * k;
+        const uint32_t* b = bits + 4 * k;
+        // The signs are the top bits of the moments' top bytes.
+        pm[k] = pack_bytes<0>(c[0], c[1], c[2], c[3]) | (pack_bytes<3>(b[0], b[1], b[2], b[3]) & 0x80808080u);
+        c = cv + 4 * k;
+        pv[k] = pack_bytes<0>(c[0], c[1], c[2], c[3]);
     }
+    if (em == 255) pm = U2{0, 0};
+    if (ev == 255) pv = U2{0, 0};
     if (e0 < n) {
-        store_codes(qm, e0, n, cm);
-        store_codes(qv, e0, n, cv);
+        store_codes(qm, e0, n, pm);
+        store_codes(qv, e0, n, pv);
         if ((threadIdx.x & 15) == 0) store_scales(scales, e0, em, ev);
     }
 }
@@ -407,29 +417,42 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const PlanTensor* __res
     const PlanTensor t = tensors[ti];
     const uint64_t g = grads.g[ti - t0];
     const A keep = t.decay ? s.keep : A(1);
-    const int64_t e0 = static_cast<int64_t>(b - t.block0) * (kState8 ? kBlock8 : kBlock32) +
-                       threadIdx.x * (kState8 ? kElems8 : kElems32);
+    const int64_t base = static_cast<int64_t>(b - t.block0) * (kState8 ? kBlock8 : kBlock32);
     if constexpr (kState8) {
-        uint32_t cm[8], cv[8], em = 0, ev = 0;
-        float p[8], gv[8], m[8], v[8];
-        load_codes(static_cast<const uint8_t*>(t.m), e0, t.n, cm);
-        load_codes(static_cast<const uint8_t*>(t.v), e0, t.n, cv);
-        if (e0 < t.n) load_scales(t.scales, e0, &em, &ev);
-        load_weight<8>(t, e0, p);
-        load_grad<8>(g, e0, t.n, gv);
-        decode_group(cm, cv, em, ev, m, v);
-        update<8, kTinyEps>(s, keep, grad_scale, p, gv, m, v);
-        store_weight<8>(t, e0, p);
-        if (e0 + 8 > t.n) {
-            // Elements past the end read as zeros and, but in a block that is not finite, stay zeros.
+        // Groups of eight neighbouring elements, a wave's groups one behind the other: 1024 elements a wave.
+        float p[kGroups8][8], gv[kGroups8][8], m[8], v[8];
+        U2 qm[kGroups8], qv[kGroups8];
+        uint32_t em[kGroups8], ev[kGroups8];
+        const int64_t e0 = base + (threadIdx.x >> 6) * (64 * kElems8) + (threadIdx.x & 63) * 8;
+        uint8_t *tm = static_cast<uint8_t*>(t.m), *tv = static_cast<uint8_t*>(t.v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (e0 + i >= t.n) m[i] = v[i] = 0.0f;
+        for (int u = 0; u < kGroups8; ++u) {
+            const int64_t e = e0 + u * 512;
+            qm[u] = load_codes(tm, e, t.n);
+            qv[u] = load_codes(tv, e, t.n);
+            em[u] = ev[u] = 0;
+            if (e < t.n) load_scales(t.scales, e, &em[u], &ev[u]);
+            load_weight<8>(t, e, p[u]);
+            load_grad<8>(g, e, t.n, gv[u]);
         }
-        const uint32_t hash = mix(mix(t.key ^ salt) + static_cast<uint32_t>(e0 >> 3));
-        encode_group(m, v, [&](int i) { return random_of(hash, i); }, e0, t.n, static_cast<uint8_t*>(t.m),
-                     static_cast<uint8_t*>(t.v), t.scales);
+        const uint32_t key = mix(t.key ^ salt);
+#pragma unroll
+        for (int u = 0; u < kGroups8; ++u) {
+            const int64_t e = e0 + u * 512;
+            decode_group(qm[u], qv[u], em[u], ev[u], m, v);
+            update<8, kTinyEps>(s, keep, grad_scale, p[u], gv[u], m, v);
+            store_weight<8>(t, e, p[u]);
+            if (e + 8 > t.n) {
+                // Elements past the end read as zeros and, but in a block that is not finite, stay zeros.
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (e + i >= t.n) m[i] = v[i] = 0.0f;
+            }
+            const uint32_t hash = mix(key + static_cast<uint32_t>(e >> 3));
+            encode_group(m, v, [&](int i) { return random_of(hash, i); }, e, t.n, tm, tv, t.scales);
+        }
     } else {
+        const int64_t e0 = base + threadIdx.x * kElems32;
         A p[kElems32], gv[kElems32], m[kElems32], v[kElems32];
         load_n<kElems32>(static_cast<const A*>(t.m), e0, t.n, m);
         load_n<kElems32>(static_cast<const A*>(t.v), e0, t.n, v);
@@ -449,13 +472,11 @@ __global__ __launch_bounds__(kThreads) void moments_decode_kernel(const uint8_t*
                                                                   bf16* __restrict__ m, bf16* __restrict__ v) {
     const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8;
     if (e0 >= n) return;
-    uint32_t cm[8], cv[8];
     float a[8], b[8];
-    load_codes(qm, e0, n, cm);
-    load_codes(qv, e0, n, cv);
+    const U2 wm = load_codes(qm, e0, n), wv = load_codes(qv, e0, n);
     uint32_t em, ev;
     load_scales(scales, e0, &em, &ev);
-    decode_group(cm, cv, em, ev, a, b);
+    decode_group(wm, wv, em, ev, a, b);
     store_n<8>(m, e0, n, a);
     store_n<8>(v, e0, n, b);
 }
@@ -695,7 +716,7 @@ extern "C" int rhp_moments_decode(const uint8_t* q_m, const uint8_t* q_v, const 
     if (int rc = check_codes("rhp_moments_decode", n, ptrs, 5)) return rc;
     if (n == 0) return 0;
     RHP_REQUIRE(element_aligned(m, RHP_BF16) && element_aligned(v, RHP_BF16), "rhp_moments_decode: unaligned output");
-    hipLaunchKernelGGL(moments_decode_kernel, dim3(static_cast<unsigned>((n + kBlock8 - 1) / kBlock8)),
+    hipLaunchKernelGGL(moments_decode_kernel, dim3(static_cast<unsigned>((n + kThreads * 8 - 1) / (kThreads * 8))),
                        dim3(kThreads), 0, stream, q_m, q_v, scales, n, static_cast<bf16*>(m), static_cast<bf16*>(v));
     return check_launch("moments_decode_kernel");
 }
@@ -707,7 +728,7 @@ extern "C" int rhp_moments_encode(const float* m, const float* v, int64_t n, uin
     if (int rc = check_codes("rhp_moments_encode", n, ptrs, 5)) return rc;
     if (n == 0) return 0;
     RHP_REQUIRE(element_aligned(m, RHP_F32) && element_aligned(v, RHP_F32), "rhp_moments_encode: unaligned input");
-    hipLaunchKernelGGL(moments_encode_kernel, dim3(static_cast<unsigned>((n + kBlock8 - 1) / kBlock8)),
+    hipLaunchKernelGGL(moments_encode_kernel, dim3(static_cast<unsigned>((n + kThreads * 8 - 1) / (kThreads * 8))),
                        dim3(kThreads), 0, stream, m, v, n, q_m, q_v, scales);
     return check_launch("moments_encode_kernel");
 }
