@@ -522,7 +522,8 @@ size_t rhp_grad_norm_workspace_bytes(int count);
  * max_norm / (out[0] + 1e-6)), what clips them (rhp_adamw_step's grad_scale).
  * Summed in double: no square overflows, and the order is fixed.  A NaN or an
  * infinity among the gradients makes the norm that, and the coefficient NaN or
- * 0.  Gradients may mix F64/F32/BF16 and need their element's alignment.
+ * 0.  Gradients may mix F64/F32/BF16 and need their element's alignment; NULL
+ * entries are skipped.
  */
 int rhp_grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel, double max_norm,
                   float* out, void* workspace, size_t workspace_bytes, hipStream_t stream);

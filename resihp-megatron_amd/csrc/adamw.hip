@@ -751,8 +751,7 @@ extern "C" int rhp_grad_norm(int count, const void* const* grads, const int* dty
     for (int i = 0; i < count; ++i) {
         RHP_REQUIRE(numel[i] >= 0 && numel[i] <= (int64_t(1) << 34), "rhp_grad_norm: element count out of range");
         RHP_REQUIRE(float_dtype(dtypes[i]), std::string("rhp_grad_norm: unsupported dtype ") + dtype_name(dtypes[i]));
-        RHP_REQUIRE(numel[i] == 0 || (grads[i] && element_aligned(grads[i], dtypes[i])),
-                    "rhp_grad_norm: a gradient is null or not aligned to its elements");
+        RHP_REQUIRE(element_aligned(grads[i], dtypes[i]), "rhp_grad_norm: a gradient is not aligned to its elements");
     }
     double* part = static_cast<double*>(workspace);
     int parts = 0;
@@ -762,9 +761,9 @@ extern "C" int rhp_grad_norm(int count, const void* const* grads, const int* dty
         uint64_t chunks = 0;
         for (int i = 0; i < ts.count; ++i) {
             ts.g[i] = tag(grads[t0 + i], dtypes[t0 + i]);
-            ts.n[i] = numel[t0 + i];
+            ts.n[i] = grads[t0 + i] ? numel[t0 + i] : 0;
             ts.chunk0[i] = static_cast<uint32_t>(chunks);
-            chunks += static_cast<uint64_t>((numel[t0 + i] + kNormChunk - 1) / kNormChunk);
+            chunks += static_cast<uint64_t>((ts.n[i] + kNormChunk - 1) / kNormChunk);
         }
         ts.chunk0[ts.count] = static_cast<uint32_t>(chunks);
         if (chunks == 0) continue;

@@ -748,10 +748,19 @@ def adam_step(params: list[torch.Tensor], grads: list[torch.Tensor | None], exp_
 # ----------------------------------------------------------------------------- layer norm
 
 
-def _norm_args(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None) -> int:
-    """Checks a norm's rows and parameters; the code of the parameters' dtype."""
+def _norm_args(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None) -> tuple[torch.device, int]:
+    """Checks a norm's rows and parameters; their device and the code of the parameters' dtype."""
+    dev = x.get_device()
+    t = weight if weight is not None else bias
+    if (dev >= 0 and x.dim() == 2 and x.shape[1] > 0 and x.is_contiguous() and t is not None
+            and (t.dtype is x.dtype or (t.dtype is torch.float32 and x.dtype is torch.bfloat16)) and t.dtype in _DT
+            and t.shape == x.shape[1:] and t.get_device() == dev and t.is_contiguous()
+            and (t is bias or bias is None or (bias.dtype is t.dtype and bias.shape == t.shape
+                                               and bias.get_device() == dev and bias.is_contiguous()))):
+        return x.device, _DT[t.dtype]   # the usual case in one condition; what fails it is named below
+    d = _need_cuda(x, weight, bias)
     _expect(x.dim() == 2 and x.shape[1] >= 1, f"x must be [rows, h], got {tuple(x.shape)}")
-    dt = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    dt = t.dtype if t is not None else x.dtype
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             _expect(tuple(t.shape) == (x.shape[1],), f"{name} must be [{x.shape[1]}], got {tuple(t.shape)}")
@@ -760,7 +769,7 @@ def _norm_args(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
             f"weight and bias of {x.dtype} rows must be {x.dtype}" +
             (" or float32" if x.dtype == torch.bfloat16 else "") + f", got {dt}")
     dtype_code(x)
-    return dtype_code_of(dt)
+    return d, dtype_code_of(dt)
 
 
 def _stat_dtype(x: torch.Tensor) -> torch.dtype:
@@ -772,13 +781,12 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """Layer norm of the rows of ``x`` [T, h]: (y, mean [T], rstd [T]), the statistics in float32 (float64
     for float64 rows), as ``layer_norm_bwd`` takes them.  ``weight`` and ``bias`` ([h]; x's dtype, or
     float32 with bfloat16 rows) may be None."""
-    dev = _need_cuda(x, weight, bias)
-    wc = _norm_args(x, weight, bias)
+    dev, wc = _norm_args(x, weight, bias)
     T, h = x.shape
     y = torch.empty_like(x)
-    mean, rstd = torch.empty(2, T, dtype=_stat_dtype(x), device=dev).unbind()
-    _call("rhp_layer_norm_fwd", dev, _ptr(x), dtype_code(x), _ptr(weight), _ptr(bias), wc, T, h, float(eps), _ptr(y),
-          _ptr(mean), _ptr(rstd))
+    mean, rstd = torch.empty((2, T), dtype=_stat_dtype(x), device=dev).unbind()
+    _call("rhp_layer_norm_fwd", dev, x.data_ptr(), _DT[x.dtype], _ptr(weight), _ptr(bias), wc, T, h, float(eps),
+          y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -789,25 +797,31 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
     """Gradients (dx, dweight, dbias) of ``layer_norm`` under ``dy``; ``dres`` is added to dx (the gradient
     that reaches x beside the norm).  What is not needed is not computed and comes back as None.  dweight
     and dbias have the weight's dtype (``dtype``, or x's, without a weight)."""
-    dev = _need_cuda(dy, x, weight, mean, rstd, dres)
+    dev, _ = _norm_args(x, weight, None)
     wd = weight.dtype if weight is not None else x.dtype if dtype is None else dtype
-    wc = _norm_args(x, weight, None)
-    _expect(wd == x.dtype or (x.dtype == torch.bfloat16 and wd == torch.float32), f"no {wd} gradients of {x.dtype} rows")
     T, h = x.shape
-    for name, t in (("dy", dy), ("dres", dres)):
-        if t is not None:
-            _expect(_rows_of(t, name, h, x.dtype) == T, f"{name} must have x's shape")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _expect(t.dtype == _stat_dtype(x) and tuple(t.shape) == (T,), f"{name} must be {_stat_dtype(x)} [{T}]")
+    st, i = _stat_dtype(x), dev.index
+    for t in (dy, dres):
+        if t is not None and not (t.dtype is x.dtype and t.shape == x.shape and t.get_device() == i and t.is_contiguous()):
+            _need_cuda(x, dy, dres)
+            raise KernelArgumentError(f"dy and dres must be {x.dtype} with x's shape, got {t.dtype} {tuple(t.shape)}")
+    for t in (mean, rstd):
+        if not (t.dtype is st and t.shape == x.shape[:1] and t.get_device() == i and t.is_contiguous()):
+            _need_cuda(x, mean, rstd)
+            raise KernelArgumentError(f"mean and rstd must be {st} [{T}], got {t.dtype} {tuple(t.shape)}")
+    if wd is not x.dtype and not (x.dtype is torch.bfloat16 and wd is torch.float32):
+        raise KernelArgumentError(f"no {wd} gradients of {x.dtype} rows")
     dx = torch.empty_like(x) if need_x else None
     dw = torch.empty(h, dtype=wd, device=dev) if need_weight else None
     db = torch.empty(h, dtype=wd, device=dev) if need_bias else None
     if not (need_x or need_weight or need_bias):
         return None, None, None
-    ws_bytes = C.lib().rhp_layer_norm_bwd_workspace_bytes(T, h, dtype_code(x)) if need_weight or need_bias else 0
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    _call("rhp_layer_norm_bwd", dev, _ptr(dy), _ptr(x), dtype_code(x), _ptr(weight), dtype_code_of(wd), _ptr(mean),
-          _ptr(rstd), _ptr(dres) if need_x else None, T, h, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
+    xc, ws, ws_bytes = _DT[x.dtype], None, 0
+    if need_weight or need_bias:
+        ws_bytes = C.lib().rhp_layer_norm_bwd_workspace_bytes(T, h, xc)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("rhp_layer_norm_bwd", dev, dy.data_ptr(), x.data_ptr(), xc, _ptr(weight), _DT[wd], mean.data_ptr(),
+          rstd.data_ptr(), _ptr(dres) if need_x else None, T, h, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
     return dx, dw, db
 
 
@@ -858,7 +872,7 @@ class AdamWPlan:
         self.shapes = [p.shape for p in params]
         self.dtypes = [p.dtype for p in params]
         self.ptrs = [p.data_ptr() for p in params]
-        numel = _int_array(ctypes.c_int64, [p.numel() for p in params])
+        self.numel = numel = _int_array(ctypes.c_int64, [p.numel() for p in params])
         size = C.lib().rhp_adamw_plan_bytes(n, numel, 8 if eight else 32)
         self.image = torch.empty(size, dtype=torch.uint8)
         addr = lambda ts: C.ptr_array([0 if t is None else t.data_ptr() for t in ts])  # noqa: E731
@@ -873,41 +887,48 @@ class AdamWPlan:
         return [p.data_ptr() for p in self.params] != self.ptrs
 
 
-def _grad_arrays(plan: AdamWPlan, grads):
-    """Pointer and dtype arrays of a plan's gradients, checked."""
-    _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
-    dev, ptrs, codes = plan.device.index, [], []
-    f64 = plan.dtypes[0] == torch.float64
-    for i, g in enumerate(grads):
-        if g is None:
-            ptrs.append(0)
-            codes.append(0)
-            continue
-        if g.get_device() != dev:
-            raise RuntimeError(f"gradient {i} is not on {plan.device}")
-        code = _DT.get(g.dtype)
-        _expect(code is not None and (code == C.F64) == f64, f"gradient {i} has dtype {g.dtype}")
-        _expect(g.shape == plan.shapes[i] and g.is_contiguous(), f"gradient {i} must be contiguous with the param's shape")
-        ptrs.append(g.data_ptr())
-        codes.append(code)
-    return C.ptr_array(ptrs), _int_array(ctypes.c_int, codes)
+class PlanGrads:
+    """A plan's gradients, checked, with the arrays that the calls of one step take.  Not kept beyond it."""
+
+    def __init__(self, plan: AdamWPlan, grads):
+        _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
+        dev, ptrs, codes = plan.device.index, [], []
+        f64 = plan.dtypes[0] is torch.float64
+        for g, shape in zip(grads, plan.shapes):
+            if g is None:
+                ptrs.append(0)
+                codes.append(0)
+                continue
+            code = _DT.get(g.dtype, -1)
+            if g.get_device() != dev or code < 0 or (code == C.F64) != f64 or g.shape != shape or not g.is_contiguous():
+                raise KernelArgumentError(
+                    f"gradient {len(ptrs)} must be contiguous with its parameter's shape, on {plan.device}, float32 or "
+                    f"bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on {g.device}")
+            ptrs.append(g.data_ptr())
+            codes.append(code)
+        self.plan, self.grads = plan, grads
+        self.any = any(ptrs)
+        self.ptrs, self.codes = C.ptr_array(ptrs), _int_array(ctypes.c_int, codes)
 
 
 def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
                step: int, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
     """One AdamW step over the plan's tensors, in place, in one launch (up to 448 tensors).
 
-    ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights); None steps with
-    zeros.  ``grad_scale``: float32 tensor of one element on the device that every gradient is multiplied
-    with.  ``step`` counts from 1.  ``seed``: of the random bits that round moments of 8 bits."""
-    garr, gcodes = _grad_arrays(plan, grads)
-    if plan.moved():
-        raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made")
+    ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights), or the plan's
+    ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device that
+    every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the random bits that round
+    moments of 8 bits."""
+    if not isinstance(grads, PlanGrads):
+        grads = PlanGrads(plan, grads)
+    if plan.moved() or grads.plan is not plan:
+        raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made, or the gradients "
+                                  "are another plan's")
     if grad_scale is not None:
         _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
-                f"grad_scale must be one float32 on {plan.device}")
-    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), garr,
-          gcodes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
+                "grad_scale must be one float32 on the plan's device")
+    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), grads.ptrs,
+          grads.codes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
           _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)
 
 
@@ -941,17 +962,29 @@ def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: tor
 def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
     """float32 [2] on the device: the 2-norm over all elements of all gradients (summed in float64), and
     min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
-    one device, None entries skipped."""
-    grads = [g for g in grads if g is not None]
-    _expect(len(grads) > 0, "grad_norm needs a gradient")
-    _expect(max_norm > 0, "max_norm must be positive")
-    dev = _need_cuda(*grads)
-    codes = _int_array(ctypes.c_int, [dtype_code(g) for g in grads])
+    one device, None entries skipped; or a plan's ``PlanGrads``."""
+    if isinstance(grads, PlanGrads):
+        dev, n, ptrs, codes, numel = grads.plan.device, len(grads.grads), grads.ptrs, grads.codes, grads.plan.numel
+        _expect(grads.any, "grad_norm needs a gradient")
+    else:
+        grads = [g for g in grads if g is not None]
+        n = len(grads)
+        _expect(n > 0, "grad_norm needs a gradient")
+        i = grads[0].get_device()
+        for g in grads:
+            if i < 0 or g.get_device() != i or not g.is_contiguous() or g.dtype not in _DT:
+                _need_cuda(*grads)
+                dtype_code(g)
+        dev = grads[0].device
+        ptrs = C.ptr_array([g.data_ptr() for g in grads])
+        codes = _int_array(ctypes.c_int, [_DT[g.dtype] for g in grads])
+        numel = _int_array(ctypes.c_int64, [g.numel() for g in grads])
+    if not max_norm > 0:
+        raise KernelArgumentError(f"max_norm must be positive, got {max_norm}")
     out = torch.empty(2, dtype=torch.float32, device=dev)
-    ws_bytes = C.lib().rhp_grad_norm_workspace_bytes(len(grads))
+    ws_bytes = C.lib().rhp_grad_norm_workspace_bytes(n)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call("rhp_grad_norm", dev, len(grads), C.ptr_array([g.data_ptr() for g in grads]), codes,
-          _int_array(ctypes.c_int64, [g.numel() for g in grads]), float(max_norm), _ptr(out), _ptr(ws), ws_bytes)
+    _call("rhp_grad_norm", dev, n, ptrs, codes, numel, float(max_norm), out.data_ptr(), ws.data_ptr(), ws_bytes)
     return out
 
 

@@ -359,9 +359,8 @@ class AdamW:
         plan = self._plan
         if plan is None or plan.moved():
             plan = self._plan = self._make_plan()
-        norm = None
-        if self.max_grad_norm is not None and any(g is not None for g in grads):
-            norm = K.grad_norm(grads, self.max_grad_norm)
+        grads = K.PlanGrads(plan, grads)
+        norm = K.grad_norm(grads, self.max_grad_norm) if self.max_grad_norm is not None and grads.any else None
         K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
                      None if norm is None else norm[1:], self.seed)
         self.step_count += 1
