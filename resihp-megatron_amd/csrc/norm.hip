@@ -30,16 +30,80 @@ constexpr int kNormWaves = kNormThreads / 64;
 __device__ __forceinline__ float rsqrt_t(float x) { return 1.0f / __builtin_sqrtf(x); }
 __device__ __forceinline__ double rsqrt_t(double x) { return 1.0 / __builtin_sqrt(x); }
 
-template <class A> __device__ __forceinline__ A wave_sum(A v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+template <int kCtrl> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
+}
+// Sum over neighbouring lanes (8, 16, 32 or 64 of them), in all of them.
+template <int kLanes> __device__ __forceinline__ float lane_sum(float v) {
+    v += dpp<0xB1>(v);                           // quad_perm [1,0,3,2]
+    v += dpp<0x4E>(v);                           // quad_perm [2,3,0,1]
+    v += dpp<0x141>(v);                          // row_half_mirror: the other four of eight
+    if constexpr (kLanes > 8) v += dpp<0x140>(v);   // row_mirror: the other eight of sixteen
+    if constexpr (kLanes > 16) v += __shfl_xor(v, 16, 64);
+    if constexpr (kLanes > 32) v += __shfl_xor(v, 32, 64);
     return v;
 }
+template <int kLanes> __device__ __forceinline__ double lane_sum(double v) {
+#pragma unroll
+    for (int d = kLanes / 2; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// ------------------------------------------------------------------ chunks of 16 bytes
+
+// A vector access needs no alignment beyond its element's, and costs the same
+// where it is aligned.
+typedef uint32_t Q __attribute__((ext_vector_type(4)));
+typedef Q Qu __attribute__((aligned(2)));
+template <class S> constexpr int kVec = 16 / static_cast<int>(sizeof(S));
+
+template <class S> struct Chunk {
+    Q q;
+    __device__ __forceinline__ void load(const S* p) { q = __builtin_nontemporal_load(reinterpret_cast<const Qu*>(p)); }
+    __device__ __forceinline__ typename Elem<S>::acc at(int j) const {
+        if constexpr (sizeof(S) == 8)
+            return __hiloint2double(static_cast<int>(q[2 * j + 1]), static_cast<int>(q[2 * j]));
+        else if constexpr (sizeof(S) == 4)
+            return __uint_as_float(q[j]);
+        else
+            return __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
+    }
+};
+template <class S> __device__ __forceinline__ void store_chunk(S* p, const typename Elem<S>::acc* v) {
+    Q q;
+    if constexpr (sizeof(S) == 8) {
+        q = {static_cast<uint32_t>(__double2loint(v[0])), static_cast<uint32_t>(__double2hiint(v[0])),
+             static_cast<uint32_t>(__double2loint(v[1])), static_cast<uint32_t>(__double2hiint(v[1]))};
+    } else if constexpr (sizeof(S) == 4) {
+        q = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    } else {
+        q = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    }
+    *reinterpret_cast<Qu*>(p) = q;
+}
+// N elements from p on, with the ordinary cache policy: what is read again.
+template <int N, class W> __device__ __forceinline__ void load_again(const W* p, typename Elem<W>::acc* v) {
+    constexpr int M = kVec<W>;
+    static_assert(M <= N && N % M == 0, "whole chunks");
+#pragma unroll
+    for (int k = 0; k < N; k += M) {
+        Chunk<W> c;
+        c.q = *reinterpret_cast<const Qu*>(p + k);
+#pragma unroll
+        for (int j = 0; j < M; ++j) v[k + j] = c.at(j);
+    }
+}
+
+// ------------------------------------------------------------------ rows of any length
+
+// One block a row, any h: the row is read again for every pass, from the
+// caches.  For float64, and for rows that are too short or too long for
+// registers (below).
 
 // Sum of v over the block's threads, in every thread; `s` holds one value a
 // wave.  Ends with all threads past their reads of `s`.
 template <class A> __device__ __forceinline__ A block_sum(A v, A* s) {
-    v = wave_sum(v);
+    v = lane_sum<64>(v);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     A t = s[0];
@@ -49,9 +113,19 @@ template <class A> __device__ __forceinline__ A block_sum(A v, A* s) {
     return t;
 }
 
-// ------------------------------------------------------------------ rows of any length
+// Calls f(first, count) for the thread's pieces of a row: whole chunks, then single elements of the rest.
+template <int N, class F> __device__ __forceinline__ void for_pieces(int h, F f) {
+    const int whole = h / N * N;
+    for (int i = threadIdx.x * N; i < whole; i += kNormThreads * N) f(i, std::integral_constant<int, N>());
+    for (int i = whole + threadIdx.x; i < h; i += kNormThreads) f(i, std::integral_constant<int, 1>());
+}
+template <int N, class S> __device__ __forceinline__ void piece(const S* p, int i, typename Elem<S>::acc* v) {
+    if constexpr (N == 1)
+        v[0] = Elem<S>::ld(p, i);
+    else
+        load_again<N>(p + i, v);
+}
 
-// One block a row, any h: the row is read three times, the last two from the caches.
 template <class S, class W>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const S* __restrict__ x, const W* __restrict__ w,
                                                                 const W* __restrict__ b, int64_t T, int h,
@@ -62,21 +136,40 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const S* __restr
     __shared__ A s[kNormWaves];
     for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
         const S* row = x + t * h;
-        A sum = 0;
-        for (int i = threadIdx.x; i < h; i += kNormThreads) sum += Elem<S>::ld(row, i);
+        A sum = 0, sq = 0;
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A v[N];
+            piece<N>(row, i, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += v[j];
+        });
         const A mu = block_sum(sum, s) / A(h);
-        A sq = 0;
-        for (int i = threadIdx.x; i < h; i += kNormThreads) {
-            const A d = Elem<S>::ld(row, i) - mu;
-            sq += d * d;
-        }
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A v[N];
+            piece<N>(row, i, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sq += (v[j] - mu) * (v[j] - mu);
+        });
         const A r = rsqrt_t(block_sum(sq, s) / A(h) + eps);
-        for (int i = threadIdx.x; i < h; i += kNormThreads) {
-            A v = (Elem<S>::ld(row, i) - mu) * r;
-            if (w) v *= static_cast<A>(Elem<W>::ld(w, i));
-            if (b) v += static_cast<A>(Elem<W>::ld(b, i));
-            Elem<S>::st(y + t * h, i, v);
-        }
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A v[N], wv[N], bv[N];
+            piece<N>(row, i, v);
+            if (w) piece<N>(w, i, wv);
+            if (b) piece<N>(b, i, bv);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[j] = (v[j] - mu) * r;
+                if (w) v[j] *= wv[j];
+                if (b) v[j] += bv[j];
+            }
+            if constexpr (N == 1)
+                Elem<S>::st(y + t * h, i, v[0]);
+            else
+                store_chunk(y + t * h + i, v);
+        });
         if (threadIdx.x == 0) {
             mean[t] = mu;
             rstd[t] = r;
@@ -84,7 +177,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const S* __restr
     }
 }
 
-// The input gradient, one block a row, any h.
+// The input gradient.
 template <class S, class W>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const W* __restrict__ w,
@@ -96,55 +189,101 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(
         const A mu = mean[t], r = rstd[t];
         const S *xr = x + t * h, *gr = dy + t * h;
         A c1 = 0, c2 = 0;
-        for (int i = threadIdx.x; i < h; i += kNormThreads) {
-            const A g = Elem<S>::ld(gr, i) * (w ? static_cast<A>(Elem<W>::ld(w, i)) : A(1));
-            c1 += g * ((Elem<S>::ld(xr, i) - mu) * r);
-            c2 += g;
-        }
+        const auto load = [&](int i, auto n, A* g, A* xh) {
+            constexpr int N = decltype(n)::value;
+            A wv[N];
+            piece<N>(gr, i, g);
+            piece<N>(xr, i, xh);
+            if (w) piece<N>(w, i, wv);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                xh[j] = (xh[j] - mu) * r;
+                if (w) g[j] *= wv[j];
+            }
+        };
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A g[N], xh[N];
+            load(i, n, g, xh);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                c1 += g[j] * xh[j];
+                c2 += g[j];
+            }
+        });
         c1 = block_sum(c1, s) / A(h);
         c2 = block_sum(c2, s) / A(h);
-        for (int i = threadIdx.x; i < h; i += kNormThreads) {
-            const A g = Elem<S>::ld(gr, i) * (w ? static_cast<A>(Elem<W>::ld(w, i)) : A(1));
-            const A xh = (Elem<S>::ld(xr, i) - mu) * r;
-            A v = r * (g - c2 - xh * c1);
-            if (dres) v += Elem<S>::ld(dres + t * h, i);
-            Elem<S>::st(dx + t * h, i, v);
-        }
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A g[N], xh[N], v[N];
+            load(i, n, g, xh);
+            if (dres) piece<N>(dres + t * h, i, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const A d = r * (g[j] - c2 - xh[j] * c1);
+                v[j] = dres ? d + v[j] : d;
+            }
+            if constexpr (N == 1)
+                Elem<S>::st(dx + t * h, i, v[0]);
+            else
+                store_chunk(dx + t * h + i, v);
+        });
     }
 }
 
-// Partial sums of dw and db over a slice of the rows: part[slice][0 | 1][h].
+// Partial sums of dw and db over a slice of the rows, a chunk of columns a lane: part[slice][0 | 1][h].  The
+// columns behind the last whole chunk go to the single lanes of the last block.
 template <class S>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_cols_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const typename Elem<S>::acc* __restrict__ mean,
     const typename Elem<S>::acc* __restrict__ rstd, int64_t T, int h, int slices,
     typename Elem<S>::acc* __restrict__ part) {
     using A = typename Elem<S>::acc;
-    __shared__ A sw[kNormWaves][64], sb[kNormWaves][64];
+    constexpr int N = kVec<S>;
+    __shared__ A sums[kNormWaves][2 * N][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = blockIdx.x * 64 + lane;
     const int64_t t0 = T * blockIdx.y / slices, t1 = T * (blockIdx.y + 1) / slices;
-    A dw = 0, db = 0;
-    if (col < h)
+    const int whole = h / N;                                 // chunks; then h % N columns on their own
+    const int c = blockIdx.x * 64 + lane;
+    A* p = part + static_cast<int64_t>(blockIdx.y) * 2 * h;
+    const auto add = [&](int col, auto n) {
+        constexpr int M = decltype(n)::value;
+        A dw[M] = {}, db[M] = {};
         for (int64_t t = t0 + wave; t < t1; t += kNormWaves) {
-            const A g = Elem<S>::ld(dy, t * h + col);
-            dw += g * ((Elem<S>::ld(x, t * h + col) - mean[t]) * rstd[t]);
-            db += g;
+            A g[M], v[M];
+            piece<M>(dy + t * h, col, g);
+            piece<M>(x + t * h, col, v);
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                dw[j] += g[j] * ((v[j] - mean[t]) * rstd[t]);
+                db[j] += g[j];
+            }
         }
-    sw[wave][lane] = dw;
-    sb[wave][lane] = db;
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            sums[wave][j][lane] = dw[j];
+            sums[wave][N + j][lane] = db[j];
+        }
+    };
+    const bool chunk = c < whole, single = !chunk && c - whole < h % N;
+    const int col = chunk ? c * N : whole * N + (c - whole);
+    if (chunk) add(col, std::integral_constant<int, N>());
+    if (single) add(col, std::integral_constant<int, 1>());
     __syncthreads();
-    if (wave == 0 && col < h) {
+    if (wave != 0 || !(chunk || single)) return;
+    for (int j = 0; j < (chunk ? N : 1); ++j) {
+        A dw = sums[0][j][lane], db = sums[0][N + j][lane];
 #pragma unroll
         for (int i = 1; i < kNormWaves; ++i) {
-            dw += sw[i][lane];
-            db += sb[i][lane];
+            dw += sums[i][j][lane];
+            db += sums[i][N + j][lane];
         }
-        A* p = part + static_cast<int64_t>(blockIdx.y) * 2 * h;
-        p[col] = dw;
-        p[h + col] = db;
+        p[col + j] = dw;
+        p[h + col + j] = db;
     }
 }
+// Column blocks of norm_bwd_cols_kernel.
+inline int col_blocks(int h, int n) { return (h / n + h % n + 63) / 64; }
 
 // dw, db = the sums of the partial rows, a column a lane: 16 waves each sum every 16th, then wave 0 their sums.
 constexpr int kReduceThreads = 1024;
@@ -172,51 +311,16 @@ __global__ __launch_bounds__(kReduceThreads) void norm_bwd_reduce_kernel(const A
 // ------------------------------------------------------------------ rows in registers
 
 // Rows of up to 2 x 16 bytes for each of up to 1024 threads are read once and
-// held in registers: TPR threads (whole waves) own a row, each of them two
-// chunks of 16 bytes, TPR * 16 bytes apart.  The blocks stay and walk the rows;
+// held in registers: TPR threads (part of a wave, or whole waves) own a row,
+// each of them two chunks of 16 bytes, TPR * 16 bytes apart.  The blocks stay and walk the rows;
 // the next row's loads are in flight while this one is reduced, and the weight
 // (and, in the backward, the columns' sums of dw and db) stay in registers from
 // row to row.
 //
 // Rows that end inside a chunk (kTail): the last chunk is the row's last 16
 // bytes, so it overlaps the one before it.  Its first `dup` elements count for
-// no sum; both threads store the same bits to them.  A vector access needs no
-// alignment beyond its element's.
-typedef uint32_t Q __attribute__((ext_vector_type(4)));
-typedef Q Qu __attribute__((aligned(2)));
+// no sum; both threads store the same bits to them.
 constexpr int kChunks = 2;
-
-template <class S> constexpr int kVec = 16 / static_cast<int>(sizeof(S));
-
-template <class S> struct Chunk {
-    Q q;
-    __device__ __forceinline__ void load(const S* p) { q = __builtin_nontemporal_load(reinterpret_cast<const Qu*>(p)); }
-    __device__ __forceinline__ float at(int j) const {
-        if constexpr (sizeof(S) == 4) return __uint_as_float(q[j]);
-        return __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
-    }
-};
-template <class S> __device__ __forceinline__ void store_chunk(S* p, const float* v) {
-    Q q;
-    if constexpr (sizeof(S) == 4)
-        q = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    else
-        q = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    *reinterpret_cast<Qu*>(p) = q;
-}
-// N parameters from p on (every block reads them once: the ordinary cache policy).
-template <int N, class W> __device__ __forceinline__ void load_params(const W* p, float* v) {
-    constexpr int M = kVec<W>;
-#pragma unroll
-    for (int k = 0; k < N; k += M) {
-        Chunk<W> c;
-        if constexpr (M <= N) {
-            c.q = *reinterpret_cast<const Qu*>(p + k);
-#pragma unroll
-            for (int j = 0; j < M; ++j) v[k + j] = c.at(j);
-        }
-    }
-}
 
 // Where a thread's chunks lie: first element, how many of its first elements
 // another chunk counts, whether it has any.
@@ -240,7 +344,7 @@ template <int N, int TPR, bool kTail> struct Place {
 // call is enough.
 template <int K, int TPR> __device__ __forceinline__ void row_sums(float (&v)[K], float (*s)[K]) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    for (int k = 0; k < K; ++k) v[k] = lane_sum<(TPR < 64 ? TPR : 64)>(v[k]);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
@@ -256,10 +360,16 @@ template <int K, int TPR> __device__ __forceinline__ void row_sums(float (&v)[K]
         }
     }
 }
+// Which of the block's rows a thread works on (the same in every lane of a wave, if a wave has only one).
+template <int TPR> __device__ __forceinline__ int group_of() {
+    const int g = static_cast<int>(threadIdx.x) / TPR;
+    if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(g);
+    return g;
+}
 
 constexpr int fwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-constexpr int bwd_threads(int tpr) { return tpr < 512 ? 512 : tpr; }
-constexpr int kFwdBlocksPerCu = 4;   // of 256 threads
+constexpr int bwd_threads(int tpr) { return tpr < 384 ? 512 : tpr == 384 ? 768 : tpr; }
+constexpr int kFwdThreadsPerCu = 1024;
 
 template <class S, class W, int TPR, bool kTail>
 __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S* __restrict__ x,
@@ -270,7 +380,7 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
                                                                         float* __restrict__ rstd) {
     constexpr int N = kVec<S>, G = fwd_threads(TPR) / TPR;
     __shared__ float red[2][fwd_threads(TPR) / 64][1];
-    const int grp = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / TPR));
+    const int grp = group_of<TPR>();
     const Place<N, TPR, kTail> at(threadIdx.x % TPR, h);
     float wv[kChunks][N], bv[kChunks][N];
     Chunk<S> cur[kChunks], nxt[kChunks];
@@ -288,8 +398,8 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
             wv[v][j] = 1.0f;
             bv[v][j] = 0.0f;
         }
-        if (w && at.on[v]) load_params<N>(w + at.off[v], wv[v]);
-        if (b && at.on[v]) load_params<N>(b + at.off[v], bv[v]);
+        if (w && at.on[v]) load_again<N>(w + at.off[v], wv[v]);
+        if (b && at.on[v]) load_again<N>(b + at.off[v], bv[v]);
     }
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < T; base += stride, t += stride) {
 #pragma unroll
@@ -341,7 +451,7 @@ template <class S> struct BwdRow {
     float mu, r;
 };
 
-template <class S, class W, int TPR, bool kTail, bool kSums>
+template <class S, class W, int TPR, bool kTail>
 __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const W* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, const S* __restrict__ dres, int64_t T, int h, S* __restrict__ dx,
@@ -349,7 +459,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     constexpr int N = kVec<S>, G = bwd_threads(TPR) / TPR;
     constexpr bool kAhead = TPR < 1024;   // 16 waves a block leave no registers for the next row
     __shared__ float red[2][bwd_threads(TPR) / 64][2];
-    const int grp = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / TPR));
+    const int grp = group_of<TPR>();
     const int i = threadIdx.x % TPR;
     const Place<N, TPR, kTail> at(i, h);
     float wv[kChunks][N], aw[kChunks][N], ab[kChunks][N];
@@ -381,7 +491,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
             wv[v][j] = 1.0f;
             aw[v][j] = ab[v][j] = 0.0f;
         }
-        if (w && at.on[v]) load_params<N>(w + at.off[v], wv[v]);
+        if (w && at.on[v]) load_again<N>(w + at.off[v], wv[v]);
     }
     int turn = 0;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < T; base += stride, t += stride, turn ^= 1) {
@@ -392,10 +502,8 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float d = cur.dy[v].at(j), xh = (cur.x[v].at(j) - cur.mu) * cur.r;
-                if constexpr (kSums) {
-                    aw[v][j] += d * xh;
-                    ab[v][j] += d;
-                }
+                aw[v][j] += d * xh;
+                ab[v][j] += d;
                 const float g = at.counts(v, j) ? d * wv[v][j] : 0.0f;
                 c[0] += g * xh;
                 c[1] += g;
@@ -423,61 +531,72 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
         else
             load(cur, t + stride);
     }
-    if constexpr (kSums) {
-        // The block's rows: the groups' sums one after the other, then a partial row each of dw and db (or
-        // the result itself, if this block had all rows).
-        if constexpr (G > 1) {
-            __shared__ float sums[2 * kChunks * N * TPR];
-            for (int g = 1; g < G; ++g) {
-                __syncthreads();
-                if (grp == g) {
+    if (!dw && !db) return;
+    // The block's rows: the sums of a wave's groups, then the waves' (or groups') one after the other, then a
+    // partial row each of dw and db (or the result itself, if this block had all rows).
+    if constexpr (TPR < 64) {
 #pragma unroll
-                    for (int v = 0; v < kChunks; ++v)
+        for (int v = 0; v < kChunks; ++v)
 #pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            sums[(v * N + j) * TPR + i] = aw[v][j];
-                            sums[((kChunks + v) * N + j) * TPR + i] = ab[v][j];
-                        }
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int d = TPR; d < 64; d *= 2) {
+                    aw[v][j] += __shfl_xor(aw[v][j], d, 64);
+                    ab[v][j] += __shfl_xor(ab[v][j], d, 64);
                 }
-                __syncthreads();
-                if (grp == 0) {
+    }
+    constexpr int kParts = TPR < 64 ? bwd_threads(TPR) / 64 : G;
+    const int mine = TPR < 64 ? static_cast<int>(threadIdx.x >> 6) : grp;
+    const bool has = TPR >= 64 || (threadIdx.x & 63) < TPR;
+    if constexpr (kParts > 1) {
+        __shared__ float sums[2 * kChunks * N * TPR];
+        for (int g = 1; g < kParts; ++g) {
+            __syncthreads();
+            if (mine == g && has) {
 #pragma unroll
-                    for (int v = 0; v < kChunks; ++v)
+                for (int v = 0; v < kChunks; ++v)
 #pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            aw[v][j] += sums[(v * N + j) * TPR + i];
-                            ab[v][j] += sums[((kChunks + v) * N + j) * TPR + i];
-                        }
+                    for (int j = 0; j < N; ++j) {
+                        sums[(v * N + j) * TPR + i] = aw[v][j];
+                        sums[((kChunks + v) * N + j) * TPR + i] = ab[v][j];
+                    }
+            }
+            __syncthreads();
+            if (mine == 0 && has) {
+#pragma unroll
+                for (int v = 0; v < kChunks; ++v)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        aw[v][j] += sums[(v * N + j) * TPR + i];
+                        ab[v][j] += sums[((kChunks + v) * N + j) * TPR + i];
+                    }
+            }
+        }
+    }
+    if (mine != 0 || !has) return;
+    float* p = part + static_cast<int64_t>(blockIdx.x) * 2 * h;
+#pragma unroll
+    for (int v = 0; v < kChunks; ++v)
+        if (at.on[v]) {
+            if (gridDim.x == 1) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (dw) Elem<W>::st(dw, at.off[v] + j, aw[v][j]);
+                    if (db) Elem<W>::st(db, at.off[v] + j, ab[v][j]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; k += 4) {
+                    store_chunk(p + at.off[v] + k, aw[v] + k);
+                    store_chunk(p + h + at.off[v] + k, ab[v] + k);
                 }
             }
         }
-        if (grp == 0) {
-            float* p = part + static_cast<int64_t>(blockIdx.x) * 2 * h;
-#pragma unroll
-            for (int v = 0; v < kChunks; ++v)
-                if (at.on[v]) {
-                    if (gridDim.x == 1) {
-#pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            if (dw) Elem<W>::st(dw, at.off[v] + j, aw[v][j]);
-                            if (db) Elem<W>::st(db, at.off[v] + j, ab[v][j]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < N; k += 4) {
-                            store_chunk(p + at.off[v] + k, aw[v] + k);
-                            store_chunk(p + h + at.off[v] + k, ab[v] + k);
-                        }
-                    }
-                }
-        }
-    }
 }
 
 constexpr int kNormMaxSlices = 256;
 inline int norm_slices(int64_t T, int h) {
-    const int64_t cols = (h + 63) / 64;
-    const int64_t want = std::max<int64_t>(1, 2048 / cols);            // about eight blocks a CU
+    const int64_t want = std::max<int64_t>(1, 2048 / ((h + 127) / 128));   // about eight blocks a CU of float64's chunks
     return static_cast<int>(std::max<int64_t>(1, std::min({want, (T + 15) / 16, int64_t(kNormMaxSlices)})));
 }
 
@@ -505,9 +624,23 @@ inline int row_threads(int dtype, int h) {
     if (dtype == RHP_F64) return 0;
     const int n = 16 / static_cast<int>(dtype_bytes(dtype));
     if (h < n || h > 2048 * n) return 0;
-    int tpr = 64;
-    while (tpr * kChunks * n < h) tpr *= 2;
-    return tpr;
+    for (int tpr : {8, 16, 32, 64, 128, 256, 384, 512})
+        if (tpr * kChunks * n >= h) return tpr;
+    return 1024;
+}
+// f(std::integral_constant<int, TPR>) for a row_threads() that is not 0.
+template <class F> int with_row_threads(int tpr, F f) {
+    switch (tpr) {
+        case 8: return f(std::integral_constant<int, 8>());
+        case 16: return f(std::integral_constant<int, 16>());
+        case 32: return f(std::integral_constant<int, 32>());
+        case 64: return f(std::integral_constant<int, 64>());
+        case 128: return f(std::integral_constant<int, 128>());
+        case 256: return f(std::integral_constant<int, 256>());
+        case 384: return f(std::integral_constant<int, 384>());
+        case 512: return f(std::integral_constant<int, 512>());
+        default: return f(std::integral_constant<int, 1024>());
+    }
 }
 
 template <class S, class W>
@@ -523,7 +656,7 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
         auto launch = [&](auto tpr) {
             constexpr int TPR = decltype(tpr)::value, B = fwd_threads(TPR), G = B / TPR;
             const dim3 grid(static_cast<unsigned>(
-                std::min<int64_t>((T + G - 1) / G, int64_t(device_cus()) * kFwdBlocksPerCu * 256 / B)));
+                std::min<int64_t>((T + G - 1) / G, int64_t(device_cus()) * std::max(1, (kFwdThreadsPerCu + B / 2) / B))));
             if (tail)
                 hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
                                    static_cast<float>(eps), yp, mp, rp);
@@ -532,14 +665,7 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
                                    static_cast<float>(eps), yp, mp, rp);
             return check_launch("norm_fwd_reg_kernel");
         };
-        switch (row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) {
-            case 64: return launch(std::integral_constant<int, 64>());
-            case 128: return launch(std::integral_constant<int, 128>());
-            case 256: return launch(std::integral_constant<int, 256>());
-            case 512: return launch(std::integral_constant<int, 512>());
-            case 1024: return launch(std::integral_constant<int, 1024>());
-            default: break;
-        }
+        if (const int tpr = row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) return with_row_threads(tpr, launch);
     }
     hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp, wp, bp, T, h,
                        static_cast<A>(eps), yp, mp, rp);
@@ -568,24 +694,15 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
         auto launch = [&](auto tpr) {
             constexpr int TPR = decltype(tpr)::value, B = bwd_threads(TPR), G = B / TPR;
             const int64_t nb = std::min<int64_t>((T + G - 1) / G, kNormMaxParts);
-            auto go = [&](auto tl, auto sm) {
-                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value, decltype(sm)::value>),
-                                   dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h,
-                                   dxp, dwp, dbp, part);
+            const auto go = [&](auto tl) {
+                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value>), dim3(static_cast<unsigned>(nb)),
+                                   dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h, dxp, dwp, dbp, part);
                 return check_launch("norm_bwd_reg_kernel");
             };
-            const int rc = sums ? (tail ? go(std::true_type(), std::true_type()) : go(std::false_type(), std::true_type()))
-                                : (tail ? go(std::true_type(), std::false_type()) : go(std::false_type(), std::false_type()));
+            const int rc = tail ? go(std::true_type()) : go(std::false_type());
             return rc || !sums || nb == 1 ? rc : reduce(static_cast<int>(nb));
         };
-        switch (row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) {
-            case 64: return launch(std::integral_constant<int, 64>());
-            case 128: return launch(std::integral_constant<int, 128>());
-            case 256: return launch(std::integral_constant<int, 256>());
-            case 512: return launch(std::integral_constant<int, 512>());
-            case 1024: return launch(std::integral_constant<int, 1024>());
-            default: break;
-        }
+        if (const int tpr = row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) return with_row_threads(tpr, launch);
     }
     if (dx) {
         hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp, mp,
@@ -594,7 +711,7 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
     }
     if (!sums) return 0;
     const int slices = norm_slices(T, h);
-    hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3((h + 63) / 64, slices), dim3(kNormThreads), 0, stream, dyp, xp, mp,
+    hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3(col_blocks(h, kVec<S>), slices), dim3(kNormThreads), 0, stream, dyp, xp, mp,
                        rp, T, h, slices, part);
     if (int rc = check_launch("norm_bwd_cols_kernel")) return rc;
     return reduce(slices);
@@ -612,6 +729,7 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
     RHP_REQUIRE(eps >= 0.0, "rhp_layer_norm_fwd: eps must not be negative");
     if (T == 0) return 0;
     RHP_REQUIRE(x && y && mean && rstd, "rhp_layer_norm_fwd: null pointer");
+    RHP_REQUIRE(x != y, "rhp_layer_norm_fwd: y must not be x");
     RHP_REQUIRE(element_aligned({x, y}, dtype) && element_aligned({w, b}, w_dtype) &&
                     element_aligned({mean, rstd}, dtype == RHP_F64 ? RHP_F64 : RHP_F32),
                 "rhp_layer_norm_fwd: a tensor is not aligned to its elements");
@@ -634,6 +752,7 @@ extern "C" int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, cons
     clear_error();
     if (int rc = check_norm("rhp_layer_norm_bwd", dtype, w_dtype, T, h)) return rc;
     RHP_REQUIRE(T == 0 || (dy && x && mean && rstd), "rhp_layer_norm_bwd: null pointer");
+    RHP_REQUIRE(T == 0 || !dx || (dx != dy && dx != x && dx != dres), "rhp_layer_norm_bwd: dx must not be an input");
     RHP_REQUIRE(dx || !dres, "rhp_layer_norm_bwd: the residual's gradient goes into dx, which is null");
     RHP_REQUIRE(element_aligned({dy, x, dres, dx}, dtype) && element_aligned({w, dw, db}, w_dtype) &&
                     element_aligned({mean, rstd}, dtype == RHP_F64 ? RHP_F64 : RHP_F32),

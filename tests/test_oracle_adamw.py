@@ -191,7 +191,7 @@ def test_grad_norm_refusals(kw, msg):
                a["max_norm"], a["out"], a["ws"], a["size"], None)
 
 
-def _norm_fwd(dtype=C.BF16, wd=C.F32, T=4, h=64, eps=1e-5, x=FAKE, y=FAKE):
+def _norm_fwd(dtype=C.BF16, wd=C.F32, T=4, h=64, eps=1e-5, x=FAKE, y=2 * FAKE):
     C.call("rhp_layer_norm_fwd", x, dtype, FAKE, FAKE, wd, T, h, eps, y, FAKE, FAKE, None)
 
 
@@ -199,7 +199,7 @@ def _norm_fwd(dtype=C.BF16, wd=C.F32, T=4, h=64, eps=1e-5, x=FAKE, y=FAKE):
     (dict(dtype=C.E4M3), "unsupported dtype"), (dict(dtype=C.F32, wd=C.BF16), "rows' dtype"),
     (dict(dtype=C.F64, wd=C.F32), "rows' dtype"), (dict(T=-1), "negative row count"), (dict(h=0), "h must be"),
     (dict(h=(1 << 28) + 1), "h must be"), (dict(eps=-1e-9), "eps"), (dict(eps=float("nan")), "eps"), (dict(x=0), "null"), (dict(y=0), "null"),
-    (dict(x=FAKE + 1), "not aligned"),
+    (dict(x=FAKE + 1), "not aligned"), (dict(y=FAKE), "must not be x"),
 ])
 def test_layer_norm_refusals(kw, msg):
     with pytest.raises(RuntimeError, match=msg):
@@ -209,9 +209,10 @@ def test_layer_norm_refusals(kw, msg):
 @pytest.mark.parametrize("kw,msg", [
     (dict(dy=0), "null"), (dict(ws=0), "workspace"), (dict(ws=FAKE + 8), "workspace"), (dict(size=16), "workspace"),
     (dict(wd=C.BF16), "rows' dtype"), (dict(dres=FAKE, dx=0), "residual's gradient"), (dict(dy=FAKE + 2), "not aligned"),
+    (dict(dx=FAKE), "must not be an input"), (dict(dres=2 * FAKE), "must not be an input"),
 ])
 def test_layer_norm_bwd_refusals(kw, msg):
-    a = dict(dy=FAKE, wd=C.F32, dres=0, dx=FAKE, ws=FAKE, size=1 << 24) | kw
+    a = dict(dy=FAKE, wd=C.F32, dres=0, dx=2 * FAKE, ws=FAKE, size=1 << 24) | kw
     with pytest.raises(RuntimeError, match=msg):
         C.call("rhp_layer_norm_bwd", a["dy"], FAKE, C.F32, FAKE, a["wd"], FAKE, FAKE, a["dres"] or None, 4, 64,
                a["dx"] or None, FAKE, FAKE, a["ws"], a["size"], None)
