@@ -477,8 +477,8 @@ int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, const void* w, 
  *   one byte an element, with scales: [ceil(numel/128)][2] bytes
  *   keys: what tells a tensor's random bits from the others' (state_bits = 8)
  *   decay: 0 for tensors without weight decay (NULL: all decay)
- * Tensors need their element's alignment.  The image holds addresses: a tensor
- * that moves needs a new one.
+ * Tensors need their element's alignment and must not overlap.  The image
+ * (8-byte aligned) holds addresses: a tensor that moves needs a new one.
  *
  * Moments in 8 bits (state_bits = 8): 128 neighbouring elements share an
  * exponent byte E; a code is a float's exponent and three mantissa bits above
@@ -498,7 +498,8 @@ int rhp_adamw_plan(int count, void* const* params, const int* dtypes, void* cons
  * pointers (NULL array or entry: a gradient of zeros), g_dtypes their dtypes
  * (F32 or BF16 whatever the weight's; F64 for F64 weights).  grad_scale:
  * device float that every gradient is multiplied with (NULL: 1), read when the
- * step runs.  step counts from 1.  The scalars are fixed when the call is
+ * step runs.  step counts from 1; betas in [0, 1), lr, eps and weight_decay not
+ * negative.  The scalars are fixed when the call is
  * enqueued, in a captured graph too.  One launch for up to 448 tensors.
  */
 int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,

@@ -53,10 +53,10 @@ def mix(x):
     return x ^ (x >> np.uint64(16))
 
 
-def random_bits(n: int, seed: int, step: int, key: int) -> np.ndarray:
-    """32 random bits for each of n elements: a hash of (seed, step, key, index)."""
+def random_bits(n: int, seed: int, step: int, key: int, first: int = 0) -> np.ndarray:
+    """32 random bits for each of n elements from index ``first`` on: a hash of (seed, step, key, index)."""
     salt = mix(int(mix(int(mix((step & M32) ^ (step >> 32))) ^ ((seed >> 32) & M32))) ^ (seed & M32))
-    i = np.arange(n, dtype=np.uint64)
+    i = np.arange(first, first + n, dtype=np.uint64)
     x = mix((mix(np.uint64(key) ^ salt) + (i >> np.uint64(3))) & np.uint64(M32))
     x = (x + (i & np.uint64(7)) * np.uint64(0x9E3779B9)) & np.uint64(M32)
     x = ((x ^ (x >> np.uint64(16))) * np.uint64(0x7FEB352D)) & np.uint64(M32)

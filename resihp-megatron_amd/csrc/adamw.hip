@@ -35,6 +35,8 @@
 #include <cmath>
 #include <cstring>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include "rhp_common.h"
 
@@ -621,11 +623,16 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
     clear_error();
     RHP_REQUIRE(count >= 0, "rhp_adamw_plan: count must be >= 0");
     RHP_REQUIRE(state_bits == 32 || state_bits == 8, "rhp_adamw_plan: the moments have 32 or 8 bits");
-    RHP_REQUIRE(image, "rhp_adamw_plan: null image");
+    RHP_REQUIRE(image && (reinterpret_cast<uintptr_t>(image) & 7) == 0, "rhp_adamw_plan: null or unaligned image");
     RHP_REQUIRE(count == 0 || (params && dtypes && exp_avg && exp_avg_sq && numel && (state_bits == 32 || (scales && keys))),
                 "rhp_adamw_plan: null array");
     uint64_t blocks = 0;
     bool any64 = false, other = false;
+    // What a step writes: two tensors on the same memory would race.
+    std::vector<std::pair<uintptr_t, uintptr_t>> written;
+    const auto writes = [&](const void* p, uint64_t bytes) {
+        if (p && bytes) written.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
+    };
     for (int i = 0; i < count; ++i) {
         RHP_REQUIRE(numel[i] >= 0 && numel[i] <= (int64_t(1) << 34), "rhp_adamw_plan: element count out of range");
         RHP_REQUIRE(float_dtype(dtypes[i]), std::string("rhp_adamw_plan: unsupported dtype ") + dtype_name(dtypes[i]));
@@ -640,7 +647,17 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
                         (state_bits == 8 || (element_aligned(exp_avg[i], st) && element_aligned(exp_avg_sq[i], st))) &&
                         (!masters || element_aligned(masters[i], RHP_F32)),
                     "rhp_adamw_plan: a tensor is not aligned to its elements");
+        const uint64_t n = static_cast<uint64_t>(numel[i]);
+        const uint64_t moment = n * (state_bits == 8 ? 1 : dtype_bytes(st));
+        writes(params[i], n * dtype_bytes(dtypes[i]));
+        if (masters) writes(masters[i], n * 4);
+        writes(exp_avg[i], moment);
+        writes(exp_avg_sq[i], moment);
+        if (state_bits == 8) writes(scales[i], (n + kScaleBlock - 1) / kScaleBlock * 2);
     }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        RHP_REQUIRE(written[i].first >= written[i - 1].second, "rhp_adamw_plan: two tensors share memory");
     RHP_REQUIRE(!(any64 && other), "rhp_adamw_plan: float64 weights need a plan of their own");
     RHP_REQUIRE(!(any64 && state_bits == 8), "rhp_adamw_plan: float64 weights have float64 moments, not 8 bits");
     RHP_REQUIRE(blocks < (uint64_t(1) << 31), "rhp_adamw_plan: too many elements in one plan");
@@ -667,12 +684,16 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
                               double weight_decay, int64_t step, const float* grad_scale, uint64_t seed,
                               hipStream_t stream) {
     clear_error();
-    RHP_REQUIRE(image && image_bytes >= sizeof(PlanHeader), "rhp_adamw_step: null or short image");
+    RHP_REQUIRE(image && image_bytes >= sizeof(PlanHeader) && (reinterpret_cast<uintptr_t>(image) & 7) == 0,
+                "rhp_adamw_step: null, unaligned or short image");
     const uint8_t* host = static_cast<const uint8_t*>(image);
     const PlanHeader& head = *reinterpret_cast<const PlanHeader*>(host);
     RHP_REQUIRE(head.magic == kPlanMagic && image_bytes >= plan_bytes(head.count, head.blocks),
                 "rhp_adamw_step: not an image of rhp_adamw_plan");
     RHP_REQUIRE(step >= 1, "rhp_adamw_step: step counts from 1");
+    RHP_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "rhp_adamw_step: betas must be in [0, 1)");
+    RHP_REQUIRE(lr >= 0.0 && eps >= 0.0 && weight_decay >= 0.0,
+                "rhp_adamw_step: lr, eps and weight_decay must not be negative");
     if (head.blocks == 0) return 0;
     RHP_REQUIRE(dev_image && aligned16(dev_image), "rhp_adamw_step: null or unaligned device image");
     RHP_REQUIRE(!grads || g_dtypes, "rhp_adamw_step: gradients without their dtypes");
@@ -704,7 +725,7 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
 }
 
 static int check_codes(const char* what, int64_t n, const void* const* ptrs, int count) {
-    RHP_REQUIRE(n >= 0 && n <= (int64_t(1) << 41), std::string(what) + ": element count out of range");
+    RHP_REQUIRE(n >= 0 && n <= (int64_t(1) << 34), std::string(what) + ": element count out of range");
     for (int i = 0; i < count; ++i) RHP_REQUIRE(n == 0 || ptrs[i], std::string(what) + ": null pointer");
     return 0;
 }

@@ -881,6 +881,7 @@ class AdamWPlan:
                _int_array(ctypes.c_uint32, keys), _int_array(ctypes.c_int, [int(bool(d)) for d in decay]),
                8 if eight else 32, self.image.data_ptr(), size)
         self.dev_image = self.image.to(self.device)
+        self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def moved(self) -> bool:
         """Whether a parameter's storage is no longer where the plan has it."""
@@ -927,6 +928,9 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     if grad_scale is not None:
         _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
                 "grad_scale must be one float32 on the plan's device")
+    if torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream and not torch.cuda.is_current_stream_capturing():
+        # Should the plan be dropped while this step runs, its memory waits for this stream too.
+        plan.dev_image.record_stream(torch.cuda.current_stream(plan.device))
     _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), grads.ptrs,
           grads.codes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
           _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)

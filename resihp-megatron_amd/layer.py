@@ -19,6 +19,7 @@ from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 from .fp8 import ACT, DH, DY, X, Fp8State
@@ -379,6 +380,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         _, need_x, need_w, need_b = ctx.needs_input_grad

@@ -305,6 +305,8 @@ class AdamW:
         for n, p in params.items():
             if not p.is_cuda:
                 raise RuntimeError(f"AdamW: parameter {n} is not on a HIP device; the fused step runs on the GPU")
+        if len({p.device for p in params.values()}) > 1:
+            raise RuntimeError("AdamW: the parameters are on different devices")
         self.params = dict(params)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.state_bits, self.max_grad_norm, self.no_decay, self.seed = state_bits, max_grad_norm, set(no_decay), seed
@@ -314,6 +316,7 @@ class AdamW:
         if f64 and (len(f64) < len(self.params) or state_bits == 8):
             raise ValueError("float64 parameters need an AdamW of their own, with 32-bit (here float64) moments")
         self._flat: dict[str, torch.Tensor] = {}
+        self._plan: K.AdamWPlan | None = None
         if not self.params:
             return
         names = list(self.params)
@@ -335,7 +338,6 @@ class AdamW:
                 self.state[n]["master"].copy_(self.params[n].detach())
         # Read-only: the step knows the buffers, a tensor put in a view's place would not be seen.
         self.state = {n: MappingProxyType(t) for n, t in self.state.items()}
-        self._plan: K.AdamWPlan | None = None
 
     def _allocate(self, key: str, names: list[str], dtype: torch.dtype) -> None:
         sizes = [self.params[n].numel() for n in names]
@@ -355,7 +357,7 @@ class AdamW:
         if not self.params:
             self.step_count += 1
             return
-        grads = [p.grad for p in self.params.values()]
+        grads = [p.grad if p.grad is None or p.grad.is_contiguous() else p.grad.contiguous() for p in self.params.values()]
         plan = self._plan
         if plan is None or plan.moved():
             plan = self._plan = self._make_plan()

@@ -276,6 +276,80 @@ def test_parameters_that_move_are_followed():
         K.adamw_step(plan, [None, None], 1e-3, (0.9, 0.999), 1e-8, 0.0, 1)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-20, 1.9e-12, 2.1e-12, 1e-3])
+def test_eps_down_to_zero(bits, eps):
+    """Second moments from subnormals up: with an eps that does not hide them the root is the exact one."""
+    n = 4096
+    p, g = seeded((n,), 1, 0.05).to(DEV), (seeded((n,), 2) * 10.0 ** torch.linspace(-21, 3, n)).to(DEV)
+    sdt = torch.uint8 if bits == 8 else torch.float32
+    m, v = torch.zeros(n, dtype=sdt, device=DEV), torch.zeros(n, dtype=sdt, device=DEV)
+    sc = [torch.zeros(n // 128, 2, dtype=torch.uint8, device=DEV)] if bits == 8 else None
+    plan = K.AdamWPlan([p], [m], [v], sc, keys=[1])
+    hyper = dict(lr=1e-3, betas=(0.9, 0.95), eps=eps, weight_decay=0.0)
+    say(f"adamw eps={eps} {bits}")
+    for step in (1, 2):
+        before, hv = _f32(p), (R.decode(*(t.cpu().numpy() for t in (m, v, sc[0]))) if bits == 8 else (_f32(m), _f32(v)))
+        K.adamw_step(plan, [g], *hyper.values(), step)
+        p64, _, v32 = _exact(before, _f32(g), *hv, hyper, step)
+        some = v32 > 0          # where a square underflows and eps is 0, m / 0 is infinite
+        assert some.mean() > 0.9
+        _weights_ok(p[torch.from_numpy(some).to(DEV)], p64[some], before[some].astype(np.float64), torch.float32)
+        assert torch.isfinite(p).all().item() == (eps > 0.0 or bool(some.all()))
+        p.copy_(torch.from_numpy(before))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_of_more_than_two_giga_elements(bits):
+    n, tail = (1 << 31) + 5000, 5000 + 128
+    say(f"adamw n={n} {bits}")
+    p = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    g = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    sdt = torch.uint8 if bits == 8 else torch.float32
+    m, v = torch.zeros(n, dtype=sdt, device=DEV), torch.zeros(n, dtype=sdt, device=DEV)
+    sc = torch.zeros(-(-n // 128), 2, dtype=torch.uint8, device=DEV) if bits == 8 else None
+    p[-tail:], g[-tail:] = seeded((tail,), 1, 0.05).to(DEV), seeded((tail,), 2).to(DEV)
+    before, hg = _f32(p[-tail:]), _f32(g[-tail:])
+    plan = K.AdamWPlan([p], [m], [v], None if sc is None else [sc], keys=[77])
+    K.adamw_step(plan, [g], *HYPER.values(), 1, seed=6)
+    z = np.zeros(tail, np.float32)
+    p64, m32, v32 = _exact(before, hg, z, z, HYPER, 1)
+    _weights_ok(p[-tail:], p64, before.astype(np.float64), torch.bfloat16)
+    if bits == 32:
+        assert np.array_equal(_f32(m[-tail:]), m32) and np.array_equal(_f32(v[-tail:]), v32)
+    else:
+        want = R.encode(m32, v32, R.random_bits(tail, 6, 1, 77, n - tail))
+        for t, e in zip((m[-tail:], v[-tail:], sc[-want[2].shape[0]:]), want):
+            assert np.array_equal(t.cpu().numpy(), e)
+    head = slice(0, n - tail)
+    for t in (p, m, v):
+        assert not torch.any(t[head].view(torch.uint8 if t.dtype == torch.uint8 else torch.int16 if t.dtype == torch.bfloat16
+                                          else torch.int32))
+    assert abs(K.grad_norm([g])[0].item() - np.sqrt((hg.astype(np.float64) ** 2).sum())) < 1e-4
+
+
+def test_gradients_with_strides_and_parameters_twice():
+    say("adamw strided gradient")
+    a, b = (moe.AdamW({"w": torch.nn.Parameter(seeded((40, 70), 1, 0.05).to(DEV))}, **HYPER) for _ in range(2))
+    g = seeded((70, 40), 2).to(DEV).t()
+    a.params["w"].grad, b.params["w"].grad = g, g.contiguous()
+    a.step()
+    b.step()
+    assert torch.equal(a.params["w"], b.params["w"])
+    p = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    twice = moe.AdamW({"a": p, "b": p})
+    p.grad = torch.ones(10, device=DEV)
+    with pytest.raises(RuntimeError, match="share memory"):
+        twice.step()
+    assert twice.step_count == 0 and torch.all(p == 0)
+
+
+def test_no_parameters():
+    opt = moe.AdamW({})
+    opt.step()
+    assert opt.step_count == 1 and opt.state_tensors() == {} and opt.buffers() == {}
+
+
 def test_refusals():
     p, g = torch.zeros(10, device=DEV), torch.zeros(10, device=DEV)
     z = lambda n, dt=torch.float32: torch.zeros(n, dtype=dt, device=DEV)  # noqa: E731

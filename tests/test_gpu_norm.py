@@ -272,6 +272,9 @@ def test_autograd_against_the_formula_and_against_differences():
     b = torch.randn(24, generator=g, dtype=torch.float64).to(DEV).requires_grad_(True)
     assert torch.autograd.gradcheck(lambda *a: layer.layer_norm(*a, 1e-3), (x, w, b))
     assert torch.autograd.gradcheck(lambda *a: layer.layer_norm(*a), (x, None, b))
+    with pytest.raises(RuntimeError, match="once_differentiable"):   # no second derivative, and it says so
+        dx, = torch.autograd.grad(layer.layer_norm(x, w, b).square().sum(), x, create_graph=True)
+        dx.sum().backward()
     # A transposed view goes in and a strided gradient comes back.
     xt = torch.randn(24, 10, generator=g, dtype=torch.float64).to(DEV).requires_grad_(True)
     y = layer.layer_norm(xt.t(), w, b)

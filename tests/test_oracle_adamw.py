@@ -102,7 +102,7 @@ def test_stochastic_rounding_follows_a_steady_gradient_where_nearest_stops():
 FAKE = 4096   # 16-byte aligned, never dereferenced: the checks come first
 
 
-def _plan(numel=(10,), dtypes=(C.BF16,), params=(FAKE,), m=(FAKE,), v=(FAKE,), scales=None, masters=None, keys=None,
+def _plan(numel=(10,), dtypes=(C.BF16,), params=(FAKE,), m=(2 * FAKE,), v=(3 * FAKE,), scales=None, masters=None, keys=None,
           bits=32, short=0):
     n = len(numel)
     num = (ctypes.c_int64 * n)(*numel)
@@ -124,9 +124,15 @@ def _plan(numel=(10,), dtypes=(C.BF16,), params=(FAKE,), m=(FAKE,), v=(FAKE,), s
     (dict(params=(FAKE + 1,)), "not aligned"),
     (dict(m=(FAKE + 2,)), "not aligned"),
     (dict(masters=(FAKE + 2,)), "not aligned"),
+    (dict(m=(FAKE + 16,)), "share memory"),
+    (dict(m=(3 * FAKE,)), "share memory"),
+    (dict(masters=(3 * FAKE + 36,)), "share memory"),
+    (dict(bits=8, scales=(3 * FAKE + 9,), keys=(1,)), "share memory"),
+    (dict(numel=(10, 10), dtypes=(C.F32,) * 2, params=(FAKE, FAKE), m=(5 * FAKE, 6 * FAKE), v=(7 * FAKE, 8 * FAKE)), "share memory"),
     (dict(short=1), "image smaller"),
-    (dict(dtypes=(C.F64,), bits=8, scales=(FAKE,), keys=(1,)), "float64 moments"),
-    (dict(numel=(10, 10), dtypes=(C.F64, C.F32), params=(FAKE,) * 2, m=(FAKE,) * 2, v=(FAKE,) * 2), "plan of their own"),
+    (dict(dtypes=(C.F64,), bits=8, scales=(4 * FAKE,), keys=(1,)), "float64 moments"),
+    (dict(numel=(10, 10), dtypes=(C.F64, C.F32), params=(FAKE, 2 * FAKE), m=(3 * FAKE, 4 * FAKE), v=(5 * FAKE, 6 * FAKE)),
+     "plan of their own"),
 ])
 def test_plan_refusals(kw, msg):
     with pytest.raises(RuntimeError, match=msg):
@@ -144,13 +150,19 @@ def test_plan_refuses_bad_counts():
                    C.ptr_array([FAKE]), None, (ctypes.c_int64 * 1)(n), None, None, 32, buf, 4096)
 
 
-def _step(image, size, grads=None, codes=None, step=1, dev=FAKE):
+def _step(image, size, grads=None, codes=None, step=1, dev=FAKE, hyper=(1e-3, 0.9, 0.999, 1e-8, 0.0)):
     C.call("rhp_adamw_step", image, dev, size, C.ptr_array(grads) if grads else None,
-           (ctypes.c_int * 1)(*codes) if codes else None, 1e-3, 0.9, 0.999, 1e-8, 0.0, step, None, 0, None)
+           (ctypes.c_int * 1)(*codes) if codes else None, *hyper, step, None, 0, None)
 
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(step=0), "counts from 1"),
+    (dict(hyper=(1e-3, 1.0, 0.999, 1e-8, 0.0)), "betas"),
+    (dict(hyper=(1e-3, 0.9, 1.0, 1e-8, 0.0)), "betas"),
+    (dict(hyper=(1e-3, -0.1, 0.9, 1e-8, 0.0)), "betas"),
+    (dict(hyper=(float("nan"), 0.9, 0.9, 1e-8, 0.0)), "must not be negative"),
+    (dict(hyper=(1e-3, 0.9, 0.9, -1e-8, 0.0)), "must not be negative"),
+    (dict(hyper=(1e-3, 0.9, 0.9, 1e-8, -0.1)), "must not be negative"),
     (dict(dev=0), "device image"),
     (dict(dev=FAKE + 8), "device image"),
     (dict(grads=(FAKE,)), "without their dtypes"),
