@@ -967,22 +967,27 @@ def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
     """float32 [2] on the device: the 2-norm over all elements of all gradients (summed in float64), and
     min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
     one device, None entries skipped; or a plan's ``PlanGrads``."""
+    grads = grads if isinstance(grads, PlanGrads) else list(grads)
     if isinstance(grads, PlanGrads):
         dev, n, ptrs, codes, numel = grads.plan.device, len(grads.grads), grads.ptrs, grads.codes, grads.plan.numel
         _expect(grads.any, "grad_norm needs a gradient")
     else:
-        grads = [g for g in grads if g is not None]
-        n = len(grads)
-        _expect(n > 0, "grad_norm needs a gradient")
-        i = grads[0].get_device()
+        ptrs, codes, numel, i, dev = [], [], [], None, None
         for g in grads:
-            if i < 0 or g.get_device() != i or not g.is_contiguous() or g.dtype not in _DT:
-                _need_cuda(*grads)
+            if g is None:
+                continue
+            if i is None:
+                i, dev = g.get_device(), g.device
+            code = _DT.get(g.dtype, -1)
+            if code < 0 or i < 0 or g.get_device() != i or not g.is_contiguous():
                 dtype_code(g)
-        dev = grads[0].device
-        ptrs = C.ptr_array([g.data_ptr() for g in grads])
-        codes = _int_array(ctypes.c_int, [_DT[g.dtype] for g in grads])
-        numel = _int_array(ctypes.c_int64, [g.numel() for g in grads])
+                _need_cuda(*[t for t in grads if t is not None])
+            ptrs.append(g.data_ptr())
+            codes.append(code)
+            numel.append(g.numel())
+        n = len(ptrs)
+        _expect(n > 0, "grad_norm needs a gradient")
+        ptrs, codes, numel = C.ptr_array(ptrs), _int_array(ctypes.c_int, codes), _int_array(ctypes.c_int64, numel)
     if not max_norm > 0:
         raise KernelArgumentError(f"max_norm must be positive, got {max_norm}")
     out = torch.empty(2, dtype=torch.float32, device=dev)
