@@ -14,6 +14,8 @@ Contents:
               bias update, training loop) plus the extensions the MI355X
               build adds (SwiGLU experts, sigmoid scoring, shared experts,
               FP8 delayed scaling).
+``adamw_ref`` numpy restatement of the AdamW step and of its 8-bit moments
+              (an extension: the reference has Adam only).
 
 Every oracle function is pinned by a check in ``tests/test_oracle_*.py``:
 the reference's own recorded float64 outputs (``tests/golden``), a closed

@@ -21,8 +21,8 @@ from resihp_megatron_amd import moe
 pytestmark = pytest.mark.gpu
 
 HYPER = dict(lr=2e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
-# None, a few, around the vectors', the blocks' of 128 and the thread blocks' (2048) ends.
-SIZES = [0, 1, 3, 4, 5, 7, 8, 9, 127, 128, 129, 1000, 2047, 2048, 2049, 6143, 40961]
+# None, a few, around the ends of vectors, blocks of 128, waves and thread blocks (1024 and 4096 elements).
+SIZES = [0, 1, 3, 4, 5, 7, 8, 9, 127, 128, 129, 511, 513, 1000, 1023, 1025, 2048, 2049, 4095, 4096, 4097, 6143, 40961]
 
 
 def _params(sizes, dtypes, seed):
@@ -526,21 +526,28 @@ def _loss(out, y):
     return ((out - y) ** 2).mean(dim=-1).sum()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("master", [False, True])
-def test_a_training_run_of_the_block(master):
-    """Norm, layer, backward, clip and step together: each iteration's update is the one that float64 AdamW makes
-    of the gradients that iteration had."""
+def test_a_training_run_of_the_block(master, bits):
+    """Norm, layer, backward, clip and step together: each iteration's update is the one that AdamW makes of the
+    gradients that iteration had, from the moments that the state stands for."""
     cfg = moe.MoEConfig(hidden=128, ffn=96, num_experts=4, top_k=2, tokens=100, dtype=torch.bfloat16, act="swiglu",
                         norm="layer", init_std=0.05, device=DEV)
     params = {k: torch.nn.Parameter(moe.init_param(cfg, s)) for k, s in moe.moe_specs(cfg).items()}
-    opt = moe.AdamW(params, **HYPER, max_grad_norm=0.1, master_weights=master, no_decay=("norm.weight", "norm.bias"))
-    say(f"training run master={master}")
+    opt = moe.AdamW(params, **HYPER, max_grad_norm=0.1, master_weights=master, no_decay=("norm.weight", "norm.bias"),
+                    state_bits=bits)
+    say(f"training run master={master} {bits}")
     for it in range(3):
         opt.zero_grad()
         x, y = moe.batch(cfg, it)
         (_loss(moe.reference_forward(cfg, params, x), y) / cfg.tokens).backward()
-        hosts = {n: (_f32(opt.state[n].get("master", p)), _f32(p.grad), _f32(opt.state[n]["exp_avg"]),
-                     _f32(opt.state[n]["exp_avg_sq"])) for n, p in params.items()}
+        hosts = {}
+        for n, p in params.items():
+            st = opt.state[n]
+            mv = R.decode(*(st[k].cpu().numpy().reshape(-1, 2) if k == "scales" else st[k].cpu().numpy().reshape(-1)
+                            for k in ("exp_avg", "exp_avg_sq", "scales"))) if bits == 8 else \
+                (_f32(st["exp_avg"]).reshape(-1), _f32(st["exp_avg_sq"]).reshape(-1))
+            hosts[n] = (_f32(st.get("master", p)).reshape(-1), _f32(p.grad).reshape(-1), *mv)
         opt.step()
         norm = np.sqrt(sum((h[1].astype(np.float64) ** 2).sum() for h in hosts.values()))
         assert abs(opt.grad_norm[0].item() - norm) <= 2.0 ** -23 * norm
@@ -548,6 +555,7 @@ def test_a_training_run_of_the_block(master):
         assert abs(scale - min(1.0, 0.1 / (norm + 1e-6))) <= 2.0 ** -23
         for n, p in params.items():
             w, g, m, v = hosts[n]
-            p64, m64, v64 = _exact(w, g, m, v, HYPER, it + 1, scale, not n.startswith("norm."))
+            p64, _, _ = _exact(w, g, m, v, HYPER, it + 1, scale, not n.startswith("norm."))
             mast = opt.state[n].get("master")
-            _weights_ok(p if mast is None else mast, p64, w.astype(np.float64), p.dtype if mast is None else torch.float32)
+            _weights_ok((p if mast is None else mast).reshape(-1), p64, w.astype(np.float64),
+                        p.dtype if mast is None else torch.float32)
