@@ -392,9 +392,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of ``x`` (with autograd), in float32 (float64 for float64) whatever
     x's dtype.  ``weight`` and ``bias``: [h] in x's dtype, or float32 with bfloat16 rows, or None."""
-    h = x.shape[-1]
-    if h == 0:
+    if x.dim() == 0 or x.shape[-1] == 0:
         raise K.KernelArgumentError("layer_norm needs at least one element a row")
+    h = x.shape[-1]
     rows = x.reshape(-1, h).contiguous()
     return _LayerNormFn.apply(float(eps), rows, None if weight is None else weight.contiguous(),
                               None if bias is None else bias.contiguous()).view(x.shape)

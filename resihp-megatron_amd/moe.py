@@ -7,8 +7,9 @@ deliberate:
 
 * ``MoEConfig`` gains fields for the extensions (SwiGLU experts, sigmoid
   scoring, shared experts, a seeded initial expert bias, Gaussian weight init
-  with a fixed std, a separate router dtype, the device).  Defaults reproduce
-  the reference configuration.
+  with a fixed std, a separate router dtype, the device, a layer norm in
+  front).  Defaults reproduce the reference configuration.
+* ``layer_norm`` and ``AdamW`` stand beside the reference's names.
 * Top-k ties go to the lowest expert id (the reference inherits torch.topk's
   unspecified order), and NaN router keys rank last.
 * Cross-GPU expert parallelism is out of scope: ``EPRuntime`` runs when the EP
@@ -305,6 +306,7 @@ class AdamW:
         for n, p in params.items():
             if not p.is_cuda:
                 raise RuntimeError(f"AdamW: parameter {n} is not on a HIP device; the fused step runs on the GPU")
+            K.dtype_code(p)
         if len({p.device for p in params.values()}) > 1:
             raise RuntimeError("AdamW: the parameters are on different devices")
         self.params = dict(params)
@@ -365,6 +367,8 @@ class AdamW:
         norm = K.grad_norm(grads, self.max_grad_norm) if self.max_grad_norm is not None and grads.any else None
         K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
                      None if norm is None else norm[1:], self.seed)
+        # The kernel writes the parameters behind torch's back: a graph that still holds them has to notice.
+        torch.autograd.graph.increment_version(plan.params)
         self.step_count += 1
         self.grad_norm = norm
 
@@ -401,8 +405,8 @@ class AdamW:
         for n, p in self.params.items():
             p.data.copy_(tensors[f"param/{n}"])
             m, v, sc = (tensors.get(f"{key}/{n}") for key in ("exp_avg", "exp_avg_sq", "scales"))
-            if m is None or v is None:
-                raise KeyError(f"no moments of {n}")
+            if m is None or v is None or (m.dtype == torch.uint8 and sc is None):
+                raise KeyError(f"the moments of {n} are not all there")
             mine = self.state[n]
             if (m.dtype == torch.uint8) != (self.state_bits == 8):
                 m, v = (t.to(p.device) for t in (m, v))
@@ -610,5 +614,5 @@ class EPRuntime:
 
 
 __all__ = ["MoEConfig", "moe_specs", "expert_of", "init_param", "update_expert_bias", "batch", "route", "expert_ffn",
-           "token_loss", "reference_forward", "reference_train", "moe_holdings", "edp_group_name", "moe_group_specs", "layer_norm",
-           "EPRuntime", "local_keys", "Adam", "AdamW", "even_split"]
+           "token_loss", "reference_forward", "reference_train", "moe_holdings", "edp_group_name", "moe_group_specs",
+           "EPRuntime", "local_keys", "Adam", "AdamW", "even_split", "layer_norm"]

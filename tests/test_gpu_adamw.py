@@ -344,6 +344,26 @@ def test_gradients_with_strides_and_parameters_twice():
     assert twice.step_count == 0 and torch.all(p == 0)
 
 
+def test_a_graph_that_holds_the_parameters_notices_the_step():
+    p = torch.nn.Parameter(torch.ones(10, device=DEV))
+    opt = moe.AdamW({"p": p})
+    y = (p * p).sum()
+    p.grad = torch.ones(10, device=DEV)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_what_a_state_lacks_is_named():
+    opt = moe.AdamW({"p": torch.nn.Parameter(torch.ones(10, device=DEV))}, state_bits=8)
+    st = dict(opt.state_tensors())
+    for key in ("exp_avg/p", "scales/p"):
+        with pytest.raises(KeyError):
+            opt.load_state_tensors({k: v for k, v in st.items() if k != key}, 1)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        moe.AdamW({"p": torch.nn.Parameter(torch.ones(10, device=DEV, dtype=torch.float16))})
+
+
 def test_no_parameters():
     opt = moe.AdamW({})
     opt.step()
@@ -493,6 +513,22 @@ def test_captured_step(bits):
         for t, s in zip(opt.state_tensors().values(), saved):
             t.copy_(s)
         K.adamw_step(opt._plan, grads, *HYPER.values(), 2, K.grad_norm(grads, 0.5)[1:], 11)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(got, state())), i
+    # The optimizer's own step, captured: each replay is one more step with the number it was captured with.
+    opt.step_count = 1
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        opt.step()
+    for i in range(3):
+        saved = state()
+        gr.replay()
+        torch.cuda.synchronize()
+        got = state()
+        for t, s in zip(opt.state_tensors().values(), saved):
+            t.copy_(s)
+        opt.step_count = 1
+        opt.step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(got, state())), i
     fresh = moe.AdamW(_params([10], (torch.float32,), 1))

@@ -315,6 +315,32 @@ def test_captured_and_replayed(T, h):
             assert all(torch.equal(a, c) for a, c in zip(out, want)), i
 
 
+def test_captured_autograd():
+    """Forward and backward of the autograd function in one graph, on inputs that no eager graph holds."""
+    x, w, b, dy, _ = (t.to(DEV) for t in _inputs(300, 520, torch.bfloat16, torch.float32, seed=4))
+    say("norm autograd graph")
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = layer.layer_norm(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        out = step()
+    for i in range(3):
+        x.copy_(_inputs(300, 520, torch.bfloat16, torch.float32, seed=30 + i)[0])
+        want = step()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want)), i
+
+
 def test_two_streams_at_once():
     say("norm on two streams")
     sets = [[t.to(DEV) for t in _inputs(2000, h, torch.bfloat16, torch.float32, seed=h)] for h in (2048, 2056)]
