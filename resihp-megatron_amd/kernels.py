@@ -888,20 +888,25 @@ class AdamWPlan:
         return [p.data_ptr() for p in self.params] != self.ptrs
 
 
+_GRAD_DT = {torch.float32: C.F32, torch.bfloat16: C.BF16}
+
+
 class PlanGrads:
     """A plan's gradients, checked, with the arrays that the calls of one step take.  Not kept beyond it."""
 
     def __init__(self, plan: AdamWPlan, grads):
         _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
+        if plan.moved():
+            raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made")
         dev, ptrs, codes = plan.device.index, [], []
-        f64 = plan.dtypes[0] is torch.float64
+        taken = {torch.float64: C.F64} if plan.dtypes[0] is torch.float64 else _GRAD_DT
         for g, shape in zip(grads, plan.shapes):
             if g is None:
                 ptrs.append(0)
                 codes.append(0)
                 continue
-            code = _DT.get(g.dtype, -1)
-            if g.get_device() != dev or code < 0 or (code == C.F64) != f64 or g.shape != shape or not g.is_contiguous():
+            code = taken.get(g.dtype)
+            if code is None or g.get_device() != dev or g.shape != shape or not g.is_contiguous():
                 raise KernelArgumentError(
                     f"gradient {len(ptrs)} must be contiguous with its parameter's shape, on {plan.device}, float32 or "
                     f"bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on {g.device}")
@@ -922,9 +927,8 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     moments of 8 bits."""
     if not isinstance(grads, PlanGrads):
         grads = PlanGrads(plan, grads)
-    if plan.moved() or grads.plan is not plan:
-        raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made, or the gradients "
-                                  "are another plan's")
+    if grads.plan is not plan:
+        raise KernelArgumentError("the gradients are another AdamW plan's")
     if grad_scale is not None:
         _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
                 "grad_scale must be one float32 on the plan's device")

@@ -359,11 +359,14 @@ class AdamW:
         if not self.params:
             self.step_count += 1
             return
-        grads = [p.grad if p.grad is None or p.grad.is_contiguous() else p.grad.contiguous() for p in self.params.values()]
+        grads = [p.grad for p in self.params.values()]
+        if self._plan is None or self._plan.moved():
+            self._plan = self._make_plan()
         plan = self._plan
-        if plan is None or plan.moved():
-            plan = self._plan = self._make_plan()
-        grads = K.PlanGrads(plan, grads)
+        try:
+            grads = K.PlanGrads(plan, grads)
+        except K.KernelArgumentError:   # gradients with strides, or what a copy does not mend
+            grads = K.PlanGrads(plan, [None if g is None else g.contiguous() for g in grads])
         norm = K.grad_norm(grads, self.max_grad_norm) if self.max_grad_norm is not None and grads.any else None
         K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
                      None if norm is None else norm[1:], self.seed)
