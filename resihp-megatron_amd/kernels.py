@@ -9,6 +9,7 @@ device.  Nothing here computes on the CPU; every entry point goes through
 
 from __future__ import annotations
 
+import array
 import collections
 import ctypes
 
@@ -830,8 +831,13 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
 MOMENT_BLOCK = 128   # neighbouring elements that share an exponent, for moments in 8 bits
 
 
-def _int_array(kind, values) -> ctypes.Array:
-    return (kind * max(1, len(values)))(*values)
+_CODES = {ctypes.c_void_p: "Q", ctypes.c_int64: "q", ctypes.c_int: "i", ctypes.c_uint32: "I"}
+_T = torch._C.TensorBase   # its methods, mapped over lists of tensors
+
+
+def _host_array(kind, values) -> ctypes.Array:
+    """A ctypes array by way of ``array`` (for 135 values 1 us instead of the 8 of ctypes' own constructor)."""
+    return (kind * max(1, len(values))).from_buffer(array.array(_CODES[kind], values or (0,)))
 
 
 class AdamWPlan:
@@ -872,20 +878,20 @@ class AdamWPlan:
         self.shapes = [p.shape for p in params]
         self.dtypes = [p.dtype for p in params]
         self.ptrs = [p.data_ptr() for p in params]
-        self.numel = numel = _int_array(ctypes.c_int64, [p.numel() for p in params])
+        self.numel = numel = _host_array(ctypes.c_int64, [p.numel() for p in params])
         size = C.lib().rhp_adamw_plan_bytes(n, numel, 8 if eight else 32)
         self.image = torch.empty(size, dtype=torch.uint8)
         addr = lambda ts: C.ptr_array([0 if t is None else t.data_ptr() for t in ts])  # noqa: E731
-        C.call("rhp_adamw_plan", n, addr(params), _int_array(ctypes.c_int, [_DT[p.dtype] for p in params]),
+        C.call("rhp_adamw_plan", n, addr(params), _host_array(ctypes.c_int, [_DT[p.dtype] for p in params]),
                addr(masters), addr(exp_avg), addr(exp_avg_sq), addr(scales) if eight else None, numel,
-               _int_array(ctypes.c_uint32, keys), _int_array(ctypes.c_int, [int(bool(d)) for d in decay]),
+               _host_array(ctypes.c_uint32, keys), _host_array(ctypes.c_int, [int(bool(d)) for d in decay]),
                8 if eight else 32, self.image.data_ptr(), size)
         self.dev_image = self.image.to(self.device)
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def moved(self) -> bool:
         """Whether a parameter's storage is no longer where the plan has it."""
-        return [p.data_ptr() for p in self.params] != self.ptrs
+        return list(map(_T.data_ptr, self.params)) != self.ptrs
 
 
 _GRAD_DT = {torch.float32: C.F32, torch.bfloat16: C.BF16}
@@ -898,23 +904,21 @@ class PlanGrads:
         _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
         if plan.moved():
             raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made")
-        dev, ptrs, codes = plan.device.index, [], []
         taken = {torch.float64: C.F64} if plan.dtypes[0] is torch.float64 else _GRAD_DT
-        for g, shape in zip(grads, plan.shapes):
-            if g is None:
-                ptrs.append(0)
-                codes.append(0)
-                continue
-            code = taken.get(g.dtype)
-            if code is None or g.get_device() != dev or g.shape != shape or not g.is_contiguous():
-                raise KernelArgumentError(
-                    f"gradient {len(ptrs)} must be contiguous with its parameter's shape, on {plan.device}, float32 or "
-                    f"bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on {g.device}")
-            ptrs.append(g.data_ptr())
-            codes.append(code)
-        self.plan, self.grads = plan, grads
-        self.any = any(ptrs)
-        self.ptrs, self.codes = C.ptr_array(ptrs), _int_array(ctypes.c_int, codes)
+        there = [g for g in grads if g is not None]
+        codes = [0 if g is None else taken.get(g.dtype) for g in grads]
+        if (None in codes or not set(map(_T.get_device, there)) <= {plan.device.index}
+                or not all(map(_T.is_contiguous, there))
+                or [shape if g is None else g.shape for g, shape in zip(grads, plan.shapes)] != plan.shapes):
+            for i, (g, shape) in enumerate(zip(grads, plan.shapes)):
+                if g is not None and (g.dtype not in taken or g.get_device() != plan.device.index or g.shape != shape
+                                      or not g.is_contiguous()):
+                    raise KernelArgumentError(
+                        f"gradient {i} must be contiguous with its parameter's shape {tuple(shape)}, on {plan.device}, "
+                        f"float32 or bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on {g.device}")
+        self.plan, self.grads, self.any = plan, grads, bool(there)
+        self.ptrs = _host_array(ctypes.c_void_p, [0 if g is None else g.data_ptr() for g in grads])
+        self.codes = _host_array(ctypes.c_int, codes)
 
 
 def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
@@ -976,22 +980,19 @@ def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
         dev, n, ptrs, codes, numel = grads.plan.device, len(grads.grads), grads.ptrs, grads.codes, grads.plan.numel
         _expect(grads.any, "grad_norm needs a gradient")
     else:
-        ptrs, codes, numel, i, dev = [], [], [], None, None
-        for g in grads:
-            if g is None:
-                continue
-            if i is None:
-                i, dev = g.get_device(), g.device
-            code = _DT.get(g.dtype, -1)
-            if code < 0 or i < 0 or g.get_device() != i or not g.is_contiguous():
-                dtype_code(g)
-                _need_cuda(*[t for t in grads if t is not None])
-            ptrs.append(g.data_ptr())
-            codes.append(code)
-            numel.append(g.numel())
-        n = len(ptrs)
+        grads = [g for g in grads if g is not None]
+        n = len(grads)
         _expect(n > 0, "grad_norm needs a gradient")
-        ptrs, codes, numel = C.ptr_array(ptrs), _int_array(ctypes.c_int, codes), _int_array(ctypes.c_int64, numel)
+        codes = [_DT.get(g.dtype) for g in grads]
+        devs = set(map(_T.get_device, grads))
+        if len(devs) > 1 or -1 in devs or None in codes or not all(map(_T.is_contiguous, grads)):
+            _need_cuda(*grads)
+            for g in grads:
+                dtype_code(g)
+        dev = grads[0].device
+        ptrs = _host_array(ctypes.c_void_p, list(map(_T.data_ptr, grads)))
+        codes = _host_array(ctypes.c_int, codes)
+        numel = _host_array(ctypes.c_int64, list(map(_T.numel, grads)))
     if not max_norm > 0:
         raise KernelArgumentError(f"max_norm must be positive, got {max_norm}")
     out = torch.empty(2, dtype=torch.float32, device=dev)
