@@ -433,6 +433,8 @@ int rhp_adam_step(int count, void* const* params, const void* const* grads, void
  *   x, y: [T,h] dtype (F64/F32/BF16), contiguous; w, b: [h] w_dtype (the rows'
  *   dtype, or F32 with BF16 rows), either may be NULL (ones, zeros); mean, rstd:
  *   [T] float (double for F64 rows), what rhp_layer_norm_bwd takes.
+ * Statistics are float: a row whose centred squares leave its range (values
+ * past about 1e18) has rstd 0.
  * y must not overlap x.  Any 1 <= h <= 2^28, any T; rows need only their
  * element's alignment.  A row's results depend on that row alone, whatever T.
  */

@@ -18,7 +18,8 @@ M32 = 0xFFFFFFFF
 def _fma(a, b, c):
     """a b + c rounded once.  Exact for float32 in float64 but for a second rounding that one value in 2^29 could
     see; in float64, the mathematics' own type here, the extra rounding does not matter."""
-    return (np.asarray(a, np.float64) * np.asarray(b, np.float64) + np.asarray(c, np.float64)).astype(np.asarray(c).dtype)
+    wide = np.asarray(a, np.float64) * np.asarray(b, np.float64) + np.asarray(c, np.float64)
+    return wide.astype(np.asarray(c).dtype)
 
 
 def update(p, g, m, v, dtype, lr, betas, eps, weight_decay, step, scale=1.0, decay=True):

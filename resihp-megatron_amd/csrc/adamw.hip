@@ -46,6 +46,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -241,7 +242,7 @@ __device__ __forceinline__ uint32_t encode_v(uint32_t bits, int base, uint32_t r
 }
 // Four bytes from the low (kByte 0) or high (3) bytes of four words.
 template <int kByte> __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    constexpr uint32_t kPair = (uint32_t(kByte) + 4) << 8 | uint32_t(kByte);       // byte of the 2nd and of the 1st operand
+    constexpr uint32_t kPair = (uint32_t(kByte) + 4) << 8 | uint32_t(kByte);   // that byte of the 2nd and of the 1st
     const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0000u | kPair);
     const uint32_t hi = __builtin_amdgcn_perm(d, c, kPair << 16 | 0x00000C0Cu);
     return lo | hi;
@@ -572,7 +573,8 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTensors ts, dou
 }
 
 // One block: the launch and 2048 loads, 4 us.  In a launch of its own, so that no counter has to be zero before a
-// call and none is shared between two.  out = [norm, min(1, max_norm / (norm + 1e-6))]; a norm that is NaN makes the coefficient NaN.
+// call and none is shared between two.  out = [norm, min(1, max_norm / (norm + 1e-6))]; a norm that is NaN makes
+// the coefficient NaN.
 __global__ __launch_bounds__(kThreads) void grad_norm_finish_kernel(const double* __restrict__ part, int n,
                                                                     double max_norm, float* __restrict__ out) {
     __shared__ double s[kThreads / 64];
@@ -639,12 +641,18 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
     RHP_REQUIRE(count >= 0, "rhp_adamw_plan: count must be >= 0");
     RHP_REQUIRE(state_bits == 32 || state_bits == 8, "rhp_adamw_plan: the moments have 32 or 8 bits");
     RHP_REQUIRE(image && (reinterpret_cast<uintptr_t>(image) & 7) == 0, "rhp_adamw_plan: null or unaligned image");
-    RHP_REQUIRE(count == 0 || (params && dtypes && exp_avg && exp_avg_sq && numel && (state_bits == 32 || (scales && keys))),
+    RHP_REQUIRE(count == 0 || (params && dtypes && exp_avg && exp_avg_sq && numel &&
+                               (state_bits == 32 || (scales && keys))),
                 "rhp_adamw_plan: null array");
     uint64_t blocks = 0;
     bool any64 = false, other = false;
     // What a step writes: two tensors on the same memory would race.
     std::vector<std::pair<uintptr_t, uintptr_t>> written;
+    try {
+        written.reserve(5 * static_cast<size_t>(count));
+    } catch (const std::exception&) {
+        return fail("rhp_adamw_plan: out of host memory");
+    }
     const auto writes = [&](const void* p, uint64_t bytes) {
         if (p && bytes) written.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
     };
@@ -652,7 +660,8 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
         RHP_REQUIRE(numel[i] >= 0 && numel[i] <= (int64_t(1) << 34), "rhp_adamw_plan: element count out of range");
         RHP_REQUIRE(float_dtype(dtypes[i]), std::string("rhp_adamw_plan: unsupported dtype ") + dtype_name(dtypes[i]));
         (dtypes[i] == RHP_F64 ? any64 : other) = true;
-        RHP_REQUIRE(!masters || !masters[i] || dtypes[i] == RHP_BF16, "rhp_adamw_plan: masters are for bfloat16 weights");
+        RHP_REQUIRE(!masters || !masters[i] || dtypes[i] == RHP_BF16,
+                    "rhp_adamw_plan: masters are for bfloat16 weights");
         blocks += static_cast<uint64_t>(blocks_of(numel[i], state_bits == 8));
         if (numel[i] == 0) continue;
         RHP_REQUIRE(params[i] && exp_avg[i] && exp_avg_sq[i] && (state_bits == 32 || scales[i]),
@@ -678,7 +687,8 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
     RHP_REQUIRE(blocks < (uint64_t(1) << 31), "rhp_adamw_plan: too many elements in one plan");
     RHP_REQUIRE(image_bytes >= plan_bytes(static_cast<uint64_t>(count), blocks),
                 "rhp_adamw_plan: image smaller than rhp_adamw_plan_bytes()");
-    PlanHeader head{kPlanMagic, static_cast<uint32_t>(count), static_cast<uint32_t>(blocks), state_bits == 8, any64, {}};
+    const PlanHeader head{kPlanMagic, static_cast<uint32_t>(count), static_cast<uint32_t>(blocks), state_bits == 8,
+                          any64, {}};
     uint8_t* out = static_cast<uint8_t*>(image);
     std::memcpy(out, &head, sizeof head);
     PlanTensor* ts = reinterpret_cast<PlanTensor*>(out + sizeof head);

@@ -620,7 +620,8 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
 
 constexpr int kNormMaxSlices = 256;
 inline int norm_slices(int64_t T, int h) {
-    const int64_t want = std::max<int64_t>(1, 2048 / ((h + 127) / 128));   // about eight blocks a CU of float64's chunks
+    // About eight blocks a CU of float64's chunks.
+    const int64_t want = std::max<int64_t>(1, 2048 / ((h + 127) / 128));
     return static_cast<int>(std::max<int64_t>(1, std::min({want, (T + 15) / 16, int64_t(kNormMaxSlices)})));
 }
 
@@ -679,8 +680,8 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
         const bool tail = h % kVec<S> != 0;
         auto launch = [&](auto tpr) {
             constexpr int TPR = decltype(tpr)::value, B = fwd_threads(TPR), G = B / TPR;
-            const dim3 grid(static_cast<unsigned>(
-                std::min<int64_t>((T + G - 1) / G, int64_t(device_cus()) * std::max(1, (kFwdThreadsPerCu + B / 2) / B))));
+            const int64_t most = int64_t(device_cus()) * std::max(1, (kFwdThreadsPerCu + B / 2) / B);
+            const dim3 grid(static_cast<unsigned>(std::min<int64_t>((T + G - 1) / G, most)));
             if (tail)
                 hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
                                    static_cast<float>(eps), yp, mp, rp);
@@ -720,8 +721,8 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
             const int64_t turns = (T + G - 1) / G;
             const int64_t nb = turns <= kOneBlockTurns ? 1 : std::min<int64_t>(turns, kNormMaxParts);
             const auto go = [&](auto tl) {
-                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value>), dim3(static_cast<unsigned>(nb)),
-                                   dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h, dxp, dwp, dbp, part);
+                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value>),
+                                   dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h, dxp, dwp, dbp, part);
                 return check_launch("norm_bwd_reg_kernel");
             };
             const int rc = tail ? go(std::true_type()) : go(std::false_type());
@@ -730,14 +731,14 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
         if (const int tpr = row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) return with_row_threads(tpr, launch);
     }
     if (dx) {
-        hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp, mp,
-                           rp, resp, T, h, dxp);
+        hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp,
+                           mp, rp, resp, T, h, dxp);
         if (int rc = check_launch("norm_bwd_rows_kernel")) return rc;
     }
     if (!sums) return 0;
     const int slices = norm_slices(T, h);
-    hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3(col_blocks(h, kVec<S>), slices), dim3(kNormThreads), 0, stream, dyp, xp, mp,
-                       rp, T, h, slices, part);
+    hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3(col_blocks(h, kVec<S>), slices), dim3(kNormThreads), 0, stream, dyp,
+                       xp, mp, rp, T, h, slices, part);
     if (int rc = check_launch("norm_bwd_cols_kernel")) return rc;
     return reduce(slices);
 }
@@ -758,10 +759,10 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
     RHP_REQUIRE(element_aligned({x, y}, dtype) && element_aligned({w, b}, w_dtype) &&
                     element_aligned({mean, rstd}, dtype == RHP_F64 ? RHP_F64 : RHP_F32),
                 "rhp_layer_norm_fwd: a tensor is not aligned to its elements");
-    if (dtype == RHP_F64) return norm_fwd<double, double>(x, w, b, T, h, eps, y, mean, rstd, stream);
-    if (dtype == RHP_F32) return norm_fwd<float, float>(x, w, b, T, h, eps, y, mean, rstd, stream);
-    if (w_dtype == RHP_F32) return norm_fwd<bf16, float>(x, w, b, T, h, eps, y, mean, rstd, stream);
-    return norm_fwd<bf16, bf16>(x, w, b, T, h, eps, y, mean, rstd, stream);
+    const auto run = [&](auto f) { return f(x, w, b, T, h, eps, y, mean, rstd, stream); };
+    if (dtype == RHP_F64) return run(norm_fwd<double, double>);
+    if (dtype == RHP_F32) return run(norm_fwd<float, float>);
+    return w_dtype == RHP_F32 ? run(norm_fwd<bf16, float>) : run(norm_fwd<bf16, bf16>);
 }
 
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
@@ -785,8 +786,8 @@ extern "C" int rhp_layer_norm_bwd(const void* dy, const void* x, int dtype, cons
     RHP_REQUIRE((!dw && !db) || (aligned16(workspace) && workspace &&
                                  workspace_bytes >= rhp_layer_norm_bwd_workspace_bytes(T, h, dtype)),
                 "rhp_layer_norm_bwd: workspace smaller than rhp_layer_norm_bwd_workspace_bytes(), null or unaligned");
-    if (dtype == RHP_F64) return norm_bwd<double, double>(dy, x, w, mean, rstd, dres, T, h, dx, dw, db, workspace, stream);
-    if (dtype == RHP_F32) return norm_bwd<float, float>(dy, x, w, mean, rstd, dres, T, h, dx, dw, db, workspace, stream);
-    if (w_dtype == RHP_F32) return norm_bwd<bf16, float>(dy, x, w, mean, rstd, dres, T, h, dx, dw, db, workspace, stream);
-    return norm_bwd<bf16, bf16>(dy, x, w, mean, rstd, dres, T, h, dx, dw, db, workspace, stream);
+    const auto run = [&](auto f) { return f(dy, x, w, mean, rstd, dres, T, h, dx, dw, db, workspace, stream); };
+    if (dtype == RHP_F64) return run(norm_bwd<double, double>);
+    if (dtype == RHP_F32) return run(norm_bwd<float, float>);
+    return w_dtype == RHP_F32 ? run(norm_bwd<bf16, float>) : run(norm_bwd<bf16, bf16>);
 }

@@ -306,8 +306,8 @@ def token_bwd(dout: torch.Tensor, dxp: torch.Tensor | None, pair_row: torch.Tens
         _expect(_rows_of(t, f"shared_dx[{i}]", h, dout.dtype) == T, "shared gradients need one row per token")
     dx = torch.empty_like(dout)
     arr = C.ptr_array([s.data_ptr() for s in shared_dx])
-    _call("rhp_token_bwd", dev, _ptr(dout) if residual else None, _ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi), _ptr(router_w),
-          dtype_code(router_w), arr, len(shared_dx), dtype_code(dout), T, h, router_w.shape[0], k, _ptr(dx))
+    _call("rhp_token_bwd", dev, _ptr(dout) if residual else None, _ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi),
+          _ptr(router_w), dtype_code(router_w), arr, len(shared_dx), dtype_code(dout), T, h, router_w.shape[0], k, _ptr(dx))
     return dx
 
 
@@ -803,7 +803,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
     T, h = x.shape
     st, i = _stat_dtype(x), dev.index
     for t in (dy, dres):
-        if t is not None and not (t.dtype is x.dtype and t.shape == x.shape and t.get_device() == i and t.is_contiguous()):
+        if t is not None and not (t.dtype is x.dtype and t.shape == x.shape and t.get_device() == i
+                                  and t.is_contiguous()):
             _need_cuda(x, dy, dres)
             raise KernelArgumentError(f"dy and dres must be {x.dtype} with x's shape, got {t.dtype} {tuple(t.shape)}")
     for t in (mean, rstd):
@@ -915,7 +916,8 @@ class PlanGrads:
                                       or not g.is_contiguous()):
                     raise KernelArgumentError(
                         f"gradient {i} must be contiguous with its parameter's shape {tuple(shape)}, on {plan.device}, "
-                        f"float32 or bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on {g.device}")
+                        f"float32 or bfloat16 (float64 with float64 weights): got {g.dtype} {tuple(g.shape)} on "
+                        f"{g.device}")
         self.plan, self.grads, self.any = plan, grads, bool(there)
         self.ptrs = _host_array(ctypes.c_void_p, [0 if g is None else g.data_ptr() for g in grads])
         self.codes = _host_array(ctypes.c_int, codes)
@@ -936,12 +938,13 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     if grad_scale is not None:
         _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
                 "grad_scale must be one float32 on the plan's device")
-    if torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream and not torch.cuda.is_current_stream_capturing():
+    if (torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream
+            and not torch.cuda.is_current_stream_capturing()):
         # Should the plan be dropped while this step runs, its memory waits for this stream too.
         plan.dev_image.record_stream(torch.cuda.current_stream(plan.device))
-    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), grads.ptrs,
-          grads.codes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
-          _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)
+    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(),
+          grads.ptrs, grads.codes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+          int(step), _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)
 
 
 def _check_moments(q_m, q_v, scales) -> int:
@@ -967,7 +970,8 @@ def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: tor
     """Writes the 8-bit codes nearest to float32 moments."""
     dev = _need_cuda(m, v, q_m, q_v, scales)
     n = _check_moments(q_m, q_v, scales)
-    _expect(m.dtype == v.dtype == torch.float32 and m.numel() == v.numel() == n, "m and v must be float32, one per code")
+    _expect(m.dtype == v.dtype == torch.float32 and m.numel() == v.numel() == n,
+            "m and v must be float32, one per code")
     _call("rhp_moments_encode", dev, _ptr(m), _ptr(v), n, _ptr(q_m), _ptr(q_v), _ptr(scales))
 
 
