@@ -785,7 +785,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     dev, wc = _norm_args(x, weight, bias)
     T, h = x.shape
     y = torch.empty_like(x)
-    mean, rstd = torch.empty((2, T), dtype=_stat_dtype(x), device=dev).unbind()
+    mean = torch.empty(T, dtype=_stat_dtype(x), device=dev)
+    rstd = torch.empty_like(mean)
     _call("rhp_layer_norm_fwd", dev, x.data_ptr(), _DT[x.dtype], _ptr(weight), _ptr(bias), wc, T, h, float(eps),
           y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
