@@ -320,29 +320,34 @@ __global__ __launch_bounds__(kReduceThreads) void norm_bwd_reduce_kernel(const A
 
 // Rows of up to 2 x 16 bytes for each of up to 1024 threads are read once and
 // held in registers: TPR threads (part of a wave, or whole waves) own a row,
-// each of them two chunks of 16 bytes, TPR * 16 bytes apart.  The blocks stay
+// each of them NV chunks of 16 bytes, TPR * 16 bytes apart.  The blocks stay
 // and walk the rows; the next row's loads are in flight while this one is
 // reduced, and the weight (and, in the backward, the columns' sums of dw and
 // db) stay in registers from row to row.  Against a block a row that reads it
 // again for each pass: 16384 x 4096 bfloat16 forward 201 -> 46 us, backward
 // (with a second read of dy and x for the columns' sums) 329 -> 100 us.
 //
-// TPR is the smallest of 8, 16, ... that holds the row: rows of 64 bfloat16 on
-// a wave each took 364 us for 64 M elements, on 8 lanes 54.
+// The shape is the smallest that holds the row, since idle lanes cost: 64 M
+// bfloat16 in rows of 64 took 364 us on a wave a row, 54 on 8 lanes; in rows
+// of 2560 52 us forward and 110 backward on 256 threads, 48 and 94 on 192; in
+// rows of 1100 68 and 137 on 128 threads, 49 and 103 on 64 with three chunks.
+// A row within a wave also spares the barriers, which shows where the backward
+// has no residual to read: rows of 2048 76 us on 128 threads, 65 on 64 with
+// four chunks (that end inside a chunk they spill; 4096-wide ones gained 8 %
+// there from four chunks and lost 2 to 14 % elsewhere: two, then).
 //
 // Rows that end inside a chunk (kTail): the last chunk is the row's last 16
 // bytes, so it overlaps the one before it.  Its first `dup` elements count for
 // no sum; both threads store the same bits to them.
-constexpr int kChunks = 2;
 
 // Where a thread's chunks lie: first element, how many of its first elements
 // another chunk counts, whether it has any.
-template <int N, int TPR, bool kTail> struct Place {
-    int off[kChunks], dup[kChunks];
-    bool on[kChunks];
+template <int N, int TPR, int NV, bool kTail> struct Place {
+    int off[NV], dup[NV];
+    bool on[NV];
     __device__ __forceinline__ Place(int i, int h) {
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v) {
+        for (int v = 0; v < NV; ++v) {
             const int c = (i + v * TPR) * N;
             on[v] = c < h;
             off[v] = kTail ? min(c, h - N) : c;
@@ -383,11 +388,11 @@ template <int TPR> __device__ __forceinline__ int group_of() {
 // Forward: blocks of 256 threads or of one row, four waves a SIMD (three: 50.5 us for 16384 x 4096, four and
 // six: 47 to 48).  Backward: one block a CU of 8 to 16 waves, which keeps the partial rows of dw and db at 256
 // (three blocks of 256 threads a CU: the same 96 us, and 7 us instead of 4.5 for the sum of 768 partial rows).
-constexpr int fwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-constexpr int bwd_threads(int tpr) { return tpr < 384 ? 512 : tpr == 384 ? 768 : tpr; }
+constexpr int fwd_threads(int tpr) { return tpr == 192 ? 384 : tpr < 256 ? 256 : tpr; }
+constexpr int bwd_threads(int tpr) { return tpr == 192 ? 576 : tpr < 384 ? 512 : tpr == 384 ? 768 : tpr; }
 constexpr int kFwdThreadsPerCu = 1024;
 
-template <class S, class W, int TPR, bool kTail>
+template <class S, class W, int TPR, int NV, bool kTail>
 __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S* __restrict__ x,
                                                                         const W* __restrict__ w,
                                                                         const W* __restrict__ b, int64_t T, int h,
@@ -397,18 +402,18 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
     constexpr int N = kVec<S>, G = fwd_threads(TPR) / TPR;
     __shared__ float red[2][fwd_threads(TPR) / 64][1];
     const int grp = group_of<TPR>();
-    const Place<N, TPR, kTail> at(threadIdx.x % TPR, h);
-    float wv[kChunks][N], bv[kChunks][N];
-    Chunk<S> cur[kChunks], nxt[kChunks];
+    const Place<N, TPR, NV, kTail> at(threadIdx.x % TPR, h);
+    float wv[NV][N], bv[NV][N];
+    Chunk<S> cur[NV], nxt[NV];
     const int64_t stride = static_cast<int64_t>(gridDim.x) * G;
     int64_t t = static_cast<int64_t>(blockIdx.x) * G + grp;
 #pragma unroll
-    for (int v = 0; v < kChunks; ++v) {
+    for (int v = 0; v < NV; ++v) {
         cur[v].q = Q{0, 0, 0, 0};
         if (at.on[v] && t < T) cur[v].load(x + t * h + at.off[v]);
     }
 #pragma unroll
-    for (int v = 0; v < kChunks; ++v) {
+    for (int v = 0; v < NV; ++v) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             wv[v][j] = 1.0f;
@@ -419,19 +424,19 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
     }
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * G; base < T; base += stride, t += stride) {
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v) {
+        for (int v = 0; v < NV; ++v) {
             nxt[v].q = Q{0, 0, 0, 0};
             if (at.on[v] && t + stride < T) nxt[v].load(x + (t + stride) * h + at.off[v]);
         }
         float sum[1] = {0.0f}, sq[1] = {0.0f};
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < N; ++j) sum[0] += at.counts(v, j) ? cur[v].at(j) : 0.0f;
         row_sums<1, TPR>(sum, red[0]);
         const float mu = sum[0] / static_cast<float>(h);
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v)
+        for (int v = 0; v < NV; ++v)
             if (at.on[v]) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
@@ -443,7 +448,7 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
         const float r = rsqrt_t(sq[0] / static_cast<float>(h) + eps);
         if (t < T) {
 #pragma unroll
-            for (int v = 0; v < kChunks; ++v)
+            for (int v = 0; v < NV; ++v)
                 if (at.on[v]) {
                     float o[N];
 #pragma unroll
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
             }
         }
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v) cur[v] = nxt[v];
+        for (int v = 0; v < NV; ++v) cur[v] = nxt[v];
     }
 }
 
@@ -467,36 +472,36 @@ constexpr int kNormMaxParts = 256;   // partial sums of dw and db (blocks of the
 // (four turns) 11.9 and 26.5 against 15.2 and 25.4.
 constexpr int kOneBlockTurns = 2;
 
-template <class S> struct BwdRow {
-    Chunk<S> x[kChunks], dy[kChunks], res[kChunks];
+template <class S, int NV> struct BwdRow {
+    Chunk<S> x[NV], dy[NV], res[NV];
     float mu, r;
 };
 
-template <class S, class W, int TPR, bool kTail>
+template <class S, class W, int TPR, int NV, bool kTail>
 __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const W* __restrict__ w, const float* __restrict__ mean,
     const float* __restrict__ rstd, const S* __restrict__ dres, int64_t T, int h, S* __restrict__ dx,
     W* __restrict__ dw, W* __restrict__ db, float* __restrict__ part) {
     constexpr int N = kVec<S>, G = bwd_threads(TPR) / TPR;
-    // 16 waves a block leave no registers for the next row (bfloat16 spills a few all the same: rows of 12288 and
-    // 16384 run at 5.9 TB/s).
-    constexpr bool kAhead = TPR < 1024;
+    // 16 waves a block, or four chunks a thread, leave no registers for the next row (16 waves of bfloat16 spill a
+    // few all the same: rows of 12288 and 16384 run at 5.9 TB/s).
+    constexpr bool kAhead = TPR < 1024 && NV < 4;
     __shared__ float red[2][bwd_threads(TPR) / 64][2];
     const int grp = group_of<TPR>();
     const int i = threadIdx.x % TPR;
-    const Place<N, TPR, kTail> at(i, h);
-    float wv[kChunks][N], aw[kChunks][N], ab[kChunks][N];
+    const Place<N, TPR, NV, kTail> at(i, h);
+    float wv[NV][N], aw[NV][N], ab[NV][N];
     const int64_t stride = static_cast<int64_t>(gridDim.x) * G;
     int64_t t = static_cast<int64_t>(blockIdx.x) * G + grp;
-    BwdRow<S> cur, nxt;
-    auto load = [&](BwdRow<S>& row, int64_t at_row) {
+    BwdRow<S, NV> cur, nxt;
+    auto load = [&](BwdRow<S, NV>& row, int64_t at_row) {
         row.mu = row.r = 0.0f;
         if (at_row < T) {
             row.mu = mean[at_row];
             row.r = rstd[at_row];
         }
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v) {
+        for (int v = 0; v < NV; ++v) {
             row.x[v].q = row.dy[v].q = row.res[v].q = Q{0, 0, 0, 0};
             if (at.on[v] && at_row < T) {
                 const int64_t e = at_row * h + at.off[v];
@@ -508,7 +513,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     };
     load(cur, t);
 #pragma unroll
-    for (int v = 0; v < kChunks; ++v) {
+    for (int v = 0; v < NV; ++v) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             wv[v][j] = 1.0f;
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
         if constexpr (kAhead) load(nxt, t + stride);
         float c[2] = {0.0f, 0.0f};   // sums of g xh and of g
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float d = cur.dy[v].at(j), xh = (cur.x[v].at(j) - cur.mu) * cur.r;
@@ -536,7 +541,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
             const float c1 = c[0] / static_cast<float>(h), c2 = c[1] / static_cast<float>(h);
             if (t < T) {
 #pragma unroll
-                for (int v = 0; v < kChunks; ++v)
+                for (int v = 0; v < NV; ++v)
                     if (at.on[v]) {
                         float o[N];
 #pragma unroll
@@ -559,7 +564,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     // partial row each of dw and db (or the result itself, if this block had all rows).
     if constexpr (TPR < 64) {
 #pragma unroll
-        for (int v = 0; v < kChunks; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < N; ++j)
 #pragma unroll
@@ -572,26 +577,26 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     const int mine = TPR < 64 ? static_cast<int>(threadIdx.x >> 6) : grp;
     const bool has = TPR >= 64 || (threadIdx.x & 63) < TPR;
     if constexpr (kParts > 1) {
-        __shared__ float sums[2 * kChunks * N * TPR];
+        __shared__ float sums[2 * NV * N * TPR];
         for (int g = 1; g < kParts; ++g) {
             __syncthreads();
             if (mine == g && has) {
 #pragma unroll
-                for (int v = 0; v < kChunks; ++v)
+                for (int v = 0; v < NV; ++v)
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
                         sums[(v * N + j) * TPR + i] = aw[v][j];
-                        sums[((kChunks + v) * N + j) * TPR + i] = ab[v][j];
+                        sums[((NV + v) * N + j) * TPR + i] = ab[v][j];
                     }
             }
             __syncthreads();
             if (mine == 0 && has) {
 #pragma unroll
-                for (int v = 0; v < kChunks; ++v)
+                for (int v = 0; v < NV; ++v)
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
                         aw[v][j] += sums[(v * N + j) * TPR + i];
-                        ab[v][j] += sums[((kChunks + v) * N + j) * TPR + i];
+                        ab[v][j] += sums[((NV + v) * N + j) * TPR + i];
                     }
             }
         }
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     if (mine != 0 || !has) return;
     float* p = part + static_cast<int64_t>(blockIdx.x) * 2 * h;
 #pragma unroll
-    for (int v = 0; v < kChunks; ++v)
+    for (int v = 0; v < NV; ++v)
         if (at.on[v]) {
             if (gridDim.x == 1) {
                 // (Where a chunk overlaps the one before, both threads summed the same rows: the same bits again.)
@@ -643,28 +648,38 @@ int check_norm(const char* what, int dtype, int w_dtype, int64_t T, int h) {
     return 0;
 }
 
-// Threads a row of the register kernels, or 0: rows shorter than a chunk, longer than 2048 chunks, float64.
-// By h and the type alone, so that a row's bits do not depend on the batch it is in.
-inline int row_threads(int dtype, int h) {
-    if (dtype == RHP_F64) return 0;
+// How the register kernels hold a row: threads and chunks a thread, 0 threads for rows shorter than a chunk or
+// longer than 2048 chunks and for float64.  By h and the type alone, so that a row's bits do not depend on the
+// batch it is in.
+struct RowShape {
+    int tpr, nv;
+};
+inline RowShape row_shape(int dtype, int h) {
+    if (dtype == RHP_F64) return {0, 0};
     const int n = 16 / static_cast<int>(dtype_bytes(dtype));
-    if (h < n || h > 2048 * n) return 0;
-    for (int tpr : {8, 16, 32, 64, 128, 256, 384, 512})
-        if (tpr * kChunks * n >= h) return tpr;
-    return 1024;
+    if (h < n || h > 2048 * n) return {0, 0};
+    for (const RowShape r : {RowShape{8, 2}, {16, 2}, {32, 2}, {64, 2}, {64, 3}, {64, 4}, {128, 2}, {192, 2}, {256, 2},
+                             {384, 2}, {512, 2}})
+        if (r.tpr * r.nv * n >= h && !(r.nv == 4 && h % n != 0)) return r;
+    return {1024, 2};
 }
-// f(std::integral_constant<int, TPR>) for a row_threads() that is not 0.
-template <class F> int with_row_threads(int tpr, F f) {
-    switch (tpr) {
-        case 8: return f(std::integral_constant<int, 8>());
-        case 16: return f(std::integral_constant<int, 16>());
-        case 32: return f(std::integral_constant<int, 32>());
-        case 64: return f(std::integral_constant<int, 64>());
-        case 128: return f(std::integral_constant<int, 128>());
-        case 256: return f(std::integral_constant<int, 256>());
-        case 384: return f(std::integral_constant<int, 384>());
-        case 512: return f(std::integral_constant<int, 512>());
-        default: return f(std::integral_constant<int, 1024>());
+// f(threads, chunks) as integral constants for a row_shape() that has threads.
+template <class F> int with_row_shape(RowShape r, F f) {
+    using Two = std::integral_constant<int, 2>;
+    switch (r.tpr) {
+        case 8: return f(std::integral_constant<int, 8>(), Two());
+        case 16: return f(std::integral_constant<int, 16>(), Two());
+        case 32: return f(std::integral_constant<int, 32>(), Two());
+        case 64:
+            if (r.nv == 3) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
+            if (r.nv == 4) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+            return f(std::integral_constant<int, 64>(), Two());
+        case 128: return f(std::integral_constant<int, 128>(), Two());
+        case 192: return f(std::integral_constant<int, 192>(), Two());
+        case 256: return f(std::integral_constant<int, 256>(), Two());
+        case 384: return f(std::integral_constant<int, 384>(), Two());
+        case 512: return f(std::integral_constant<int, 512>(), Two());
+        default: return f(std::integral_constant<int, 1024>(), Two());
     }
 }
 
@@ -678,19 +693,20 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
     A *mp = static_cast<A*>(mean), *rp = static_cast<A*>(rstd);
     if constexpr (sizeof(S) < 8) {
         const bool tail = h % kVec<S> != 0;
-        auto launch = [&](auto tpr) {
-            constexpr int TPR = decltype(tpr)::value, B = fwd_threads(TPR), G = B / TPR;
+        auto launch = [&](auto tpr, auto chunks) {
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = fwd_threads(TPR), G = B / TPR;
             const int64_t most = int64_t(device_cus()) * std::max(1, (kFwdThreadsPerCu + B / 2) / B);
             const dim3 grid(static_cast<unsigned>(std::min<int64_t>((T + G - 1) / G, most)));
             if (tail)
-                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
+                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, NV, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
                                    static_cast<float>(eps), yp, mp, rp);
             else
-                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, false>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
+                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, NV, false>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
                                    static_cast<float>(eps), yp, mp, rp);
             return check_launch("norm_fwd_reg_kernel");
         };
-        if (const int tpr = row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) return with_row_threads(tpr, launch);
+        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h);
+        if (shape.tpr) return with_row_shape(shape, launch);
     }
     hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp, wp, bp, T, h,
                        static_cast<A>(eps), yp, mp, rp);
@@ -716,19 +732,20 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
     if (T == 0) return sums ? reduce(0) : 0;
     if constexpr (sizeof(S) < 8) {
         const bool tail = h % kVec<S> != 0;
-        auto launch = [&](auto tpr) {
-            constexpr int TPR = decltype(tpr)::value, B = bwd_threads(TPR), G = B / TPR;
+        auto launch = [&](auto tpr, auto chunks) {
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = bwd_threads(TPR), G = B / TPR;
             const int64_t turns = (T + G - 1) / G;
             const int64_t nb = turns <= kOneBlockTurns ? 1 : std::min<int64_t>(turns, kNormMaxParts);
             const auto go = [&](auto tl) {
-                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, decltype(tl)::value>),
+                hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, NV, decltype(tl)::value>),
                                    dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h, dxp, dwp, dbp, part);
                 return check_launch("norm_bwd_reg_kernel");
             };
             const int rc = tail ? go(std::true_type()) : go(std::false_type());
             return rc || !sums || nb == 1 ? rc : reduce(static_cast<int>(nb));
         };
-        if (const int tpr = row_threads(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h)) return with_row_threads(tpr, launch);
+        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h);
+        if (shape.tpr) return with_row_shape(shape, launch);
     }
     if (dx) {
         hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp,
@@ -767,7 +784,7 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
 
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
     if (T < 0 || h <= 0) return 0;
-    const int64_t parts = row_threads(dtype, h) ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
+    const int64_t parts = row_shape(dtype, h).tpr ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
                                                 : norm_slices(T, h);
     return static_cast<size_t>(parts) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
 }

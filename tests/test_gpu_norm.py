@@ -22,8 +22,8 @@ HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24, torch.float64: 2.0
 TYPES = [(torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
          (torch.float64, torch.float64)]
 # One element to rows longer than any register holds; odd sizes, sizes around the vectors' and the waves' ends.
-HIDDEN = [1, 2, 3, 7, 8, 9, 63, 64, 65, 127, 255, 256, 257, 511, 512, 1000, 1023, 1365, 2048, 2049, 4096, 4099, 5120,
-          8192, 8200, 10007, 16384, 16392, 20001]
+HIDDEN = [1, 2, 3, 7, 8, 9, 63, 64, 65, 127, 255, 256, 257, 511, 512, 700, 1000, 1023, 1365, 1400, 1801, 2048, 2049,
+          2560, 4096, 4099, 5001, 5120, 6001, 8192, 8200, 10007, 16384, 16392, 20001]
 
 
 def _unit(dtype):
@@ -129,7 +129,7 @@ def test_row_counts(T, h, dt, wdt):
     assert all(torch.equal(a, c) for a, c in zip(got, again)), "the same call twice"
 
 
-@pytest.mark.parametrize("h", [8, 64, 333, 1024, 4096, 9000])
+@pytest.mark.parametrize("h", [8, 64, 333, 1024, 1400, 2048, 2301, 4096, 9000])
 def test_a_row_keeps_its_bits_in_any_batch(h):
     x, w, b, dy, dres = (t.to(DEV) for t in _inputs(600, h, torch.bfloat16, torch.float32, seed=3))
     say(f"norm batch independence h={h}")
