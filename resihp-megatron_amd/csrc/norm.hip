@@ -333,8 +333,9 @@ __global__ __launch_bounds__(kReduceThreads) void norm_bwd_reduce_kernel(const A
 // rows of 1100 68 and 137 on 128 threads, 49 and 103 on 64 with three chunks.
 // A row within a wave also spares the barriers, which shows where the backward
 // has no residual to read: rows of 2048 76 us on 128 threads, 65 on 64 with
-// four chunks (that end inside a chunk they spill; 4096-wide ones gained 8 %
-// there from four chunks and lost 2 to 14 % elsewhere: two, then).
+// four chunks.  With a residual both take 94, and of few rows the four chunks
+// 2.5 us longer; rows that end inside a chunk spill, and 4096-wide ones gained
+// 8 % without a residual and lost 2 to 14 % elsewhere: two chunks, then.
 //
 // Rows that end inside a chunk (kTail): the last chunk is the row's last 16
 // bytes, so it overlaps the one before it.  Its first `dup` elements count for
@@ -577,26 +578,33 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     const int mine = TPR < 64 ? static_cast<int>(threadIdx.x >> 6) : grp;
     const bool has = TPR >= 64 || (threadIdx.x & 63) < TPR;
     if constexpr (kParts > 1) {
-        __shared__ float sums[2 * NV * N * TPR];
-        for (int g = 1; g < kParts; ++g) {
+        // In pairs: half of the parts leave theirs in LDS, the other half adds it; parts that had no row are left out.
+        const int64_t rows = T - static_cast<int64_t>(blockIdx.x) * G, lived = (rows * TPR + 63) / 64;
+        const int live = static_cast<int>(min(TPR < 64 ? lived : rows, static_cast<int64_t>(kParts)));
+        __shared__ __align__(16) float4 sums[kParts / 2][2 * NV * N / 4 * TPR];
+        for (int s = 1; s < live; s *= 2) {
             __syncthreads();
-            if (mine == g && has) {
+            float4* slot = sums[mine / (2 * s) % (kParts / 2)];
+            if (mine % (2 * s) == s && mine < live && has) {
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        sums[(v * N + j) * TPR + i] = aw[v][j];
-                        sums[((NV + v) * N + j) * TPR + i] = ab[v][j];
+                    for (int j = 0; j < N; j += 4) {
+                        const int q = (v * N + j) / 4;
+                        slot[q * TPR + i] = make_float4(aw[v][j], aw[v][j + 1], aw[v][j + 2], aw[v][j + 3]);
+                        slot[(NV * N / 4 + q) * TPR + i] = make_float4(ab[v][j], ab[v][j + 1], ab[v][j + 2], ab[v][j + 3]);
                     }
             }
             __syncthreads();
-            if (mine == 0 && has) {
+            if (mine % (2 * s) == 0 && mine + s < live && has) {
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        aw[v][j] += sums[(v * N + j) * TPR + i];
-                        ab[v][j] += sums[((NV + v) * N + j) * TPR + i];
+                    for (int j = 0; j < N; j += 4) {
+                        const int q = (v * N + j) / 4;
+                        const float4 a = slot[q * TPR + i], b = slot[(NV * N / 4 + q) * TPR + i];
+                        aw[v][j] += a.x, aw[v][j + 1] += a.y, aw[v][j + 2] += a.z, aw[v][j + 3] += a.w;
+                        ab[v][j] += b.x, ab[v][j + 1] += b.y, ab[v][j + 2] += b.z, ab[v][j + 3] += b.w;
                     }
             }
         }
@@ -649,18 +657,18 @@ int check_norm(const char* what, int dtype, int w_dtype, int64_t T, int h) {
 }
 
 // How the register kernels hold a row: threads and chunks a thread, 0 threads for rows shorter than a chunk or
-// longer than 2048 chunks and for float64.  By h and the type alone, so that a row's bits do not depend on the
-// batch it is in.
+// longer than 2048 chunks and for float64.  By h and the type alone (and whether the backward has a residual), so
+// that a row's bits do not depend on the batch it is in.  four: whether four chunks a thread pay.
 struct RowShape {
     int tpr, nv;
 };
-inline RowShape row_shape(int dtype, int h) {
+inline RowShape row_shape(int dtype, int h, bool four) {
     if (dtype == RHP_F64) return {0, 0};
     const int n = 16 / static_cast<int>(dtype_bytes(dtype));
     if (h < n || h > 2048 * n) return {0, 0};
     for (const RowShape r : {RowShape{8, 2}, {16, 2}, {32, 2}, {64, 2}, {64, 3}, {64, 4}, {128, 2}, {192, 2}, {256, 2},
                              {384, 2}, {512, 2}})
-        if (r.tpr * r.nv * n >= h && !(r.nv == 4 && h % n != 0)) return r;
+        if (r.tpr * r.nv * n >= h && (r.nv < 4 || (four && h % n == 0))) return r;
     return {1024, 2};
 }
 // f(threads, chunks) as integral constants for a row_shape() that has threads.
@@ -683,6 +691,13 @@ template <class F> int with_row_shape(RowShape r, F f) {
     }
 }
 
+// f(whether rows end inside a chunk); rows of four chunks a thread do not (row_shape).
+template <int NV, class F> int with_tail(bool tail, F f) {
+    if constexpr (NV < 4)
+        if (tail) return f(std::true_type());
+    return f(std::false_type());
+}
+
 template <class S, class W>
 int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, double eps, void* y, void* mean,
              void* rstd, hipStream_t stream) {
@@ -692,20 +707,19 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
     S* yp = static_cast<S*>(y);
     A *mp = static_cast<A*>(mean), *rp = static_cast<A*>(rstd);
     if constexpr (sizeof(S) < 8) {
-        const bool tail = h % kVec<S> != 0;
         auto launch = [&](auto tpr, auto chunks) {
-            constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = fwd_threads(TPR), G = B / TPR;
+            constexpr int TPR = decltype(tpr)::value, B = fwd_threads(TPR), G = B / TPR;
+            constexpr int NV = std::min<int>(decltype(chunks)::value, 3);   // four are the backward's
             const int64_t most = int64_t(device_cus()) * std::max(1, (kFwdThreadsPerCu + B / 2) / B);
             const dim3 grid(static_cast<unsigned>(std::min<int64_t>((T + G - 1) / G, most)));
-            if (tail)
-                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, NV, true>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
-                                   static_cast<float>(eps), yp, mp, rp);
-            else
-                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, NV, false>), grid, dim3(B), 0, stream, xp, wp, bp, T, h,
-                                   static_cast<float>(eps), yp, mp, rp);
-            return check_launch("norm_fwd_reg_kernel");
+            const auto go = [&](auto tl) {
+                hipLaunchKernelGGL((norm_fwd_reg_kernel<S, W, TPR, NV, decltype(tl)::value>), grid, dim3(B), 0, stream,
+                                   xp, wp, bp, T, h, static_cast<float>(eps), yp, mp, rp);
+                return check_launch("norm_fwd_reg_kernel");
+            };
+            return with_tail<NV>(h % kVec<S> != 0, go);
         };
-        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h);
+        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h, false);
         if (shape.tpr) return with_row_shape(shape, launch);
     }
     hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp, wp, bp, T, h,
@@ -731,20 +745,20 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
     };
     if (T == 0) return sums ? reduce(0) : 0;
     if constexpr (sizeof(S) < 8) {
-        const bool tail = h % kVec<S> != 0;
         auto launch = [&](auto tpr, auto chunks) {
             constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = bwd_threads(TPR), G = B / TPR;
             const int64_t turns = (T + G - 1) / G;
             const int64_t nb = turns <= kOneBlockTurns ? 1 : std::min<int64_t>(turns, kNormMaxParts);
             const auto go = [&](auto tl) {
                 hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, NV, decltype(tl)::value>),
-                                   dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h, dxp, dwp, dbp, part);
+                                   dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h,
+                                   dxp, dwp, dbp, part);
                 return check_launch("norm_bwd_reg_kernel");
             };
-            const int rc = tail ? go(std::true_type()) : go(std::false_type());
+            const int rc = with_tail<NV>(h % kVec<S> != 0, go);
             return rc || !sums || nb == 1 ? rc : reduce(static_cast<int>(nb));
         };
-        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h);
+        const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h, !dres);
         if (shape.tpr) return with_row_shape(shape, launch);
     }
     if (dx) {
@@ -784,7 +798,7 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
 
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
     if (T < 0 || h <= 0) return 0;
-    const int64_t parts = row_shape(dtype, h).tpr ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
+    const int64_t parts = row_shape(dtype, h, false).tpr ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
                                                 : norm_slices(T, h);
     return static_cast<size_t>(parts) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
 }
