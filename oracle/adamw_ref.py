@@ -15,13 +15,6 @@ BLOCK = 128
 M32 = 0xFFFFFFFF
 
 
-def _fma(a, b, c):
-    """a b + c rounded once.  Exact for float32 in float64 but for a second rounding that one value in 2^29 could
-    see; in float64, the mathematics' own type here, the extra rounding does not matter."""
-    wide = np.asarray(a, np.float64) * np.asarray(b, np.float64) + np.asarray(c, np.float64)
-    return wide.astype(np.asarray(c).dtype)
-
-
 def update(p, g, m, v, dtype, lr, betas, eps, weight_decay, step, scale=1.0, decay=True):
     """New (p, m, v) as arrays of ``dtype``; ``scale`` multiplies the gradient."""
     t = np.dtype(dtype).type
@@ -30,8 +23,8 @@ def update(p, g, m, v, dtype, lr, betas, eps, weight_decay, step, scale=1.0, dec
     g, m, v = (np.asarray(x).astype(dtype) for x in (g, m, v))
     with np.errstate(all="ignore"):
         g = g * t(scale)
-        m = _fma(g, c1, m * t(b1))
-        v = _fma(g * c2, g, v * t(b2))
+        m = m * t(b1) + g * c1
+        v = v * t(b2) + (g * c2) * g
     return weight(p, m, v, dtype, lr, betas, eps, weight_decay, step, decay), m, v
 
 

@@ -11,10 +11,10 @@
 //   p = (1 - lr wd) p - (lr / bc1) * (m / (sqrt(v) / sqrt(bc2) + eps))
 //   bc1 = 1 - b1^step, bc2 = 1 - b2^step
 //
-// in float (double for double weights), one operation at a time (no fused
-// multiply-adds: what a moment rounds to in 8 bits then does not depend on
-// how the compiler contracts them); the weight is rounded once, when it is
-// stored.
+// in float (double for double weights), the moments one operation at a time
+// (no fused multiply-adds: what a moment rounds to in 8 bits is then the same
+// wherever these lines are evaluated in float); the weight is rounded once,
+// when it is stored.
 //
 // Moments in 8 bits.  128 neighbouring elements share the exponent E of the
 // largest of them (one byte a moment).  A code is the float's exponent and its
@@ -373,8 +373,8 @@ __device__ __forceinline__ void update(const Scalars<A>& s, A keep, const float*
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        m[i] = fma_of(g[i], s.c1, m[i] * s.b1);
-        v[i] = fma_of(g[i] * s.c2, g[i], v[i] * s.b2);
+        m[i] = m[i] * s.b1 + g[i] * s.c1;
+        v[i] = v[i] * s.b2 + (g[i] * s.c2) * g[i];
         const A d = fma_of(sqrt_of<kTinyEps>(v[i]), s.ibc2s, s.eps);
         p[i] = fma_of(-s.a, quotient<kTinyEps>(m[i], d), p[i] * keep);
     }
