@@ -33,8 +33,8 @@
 // The step is bound by HBM: with float32 masters and moments 28 bytes a
 // bfloat16 weight (0.57 G of them: 16.0 GB in 2.65 to 2.9 ms, 5.5 to 6.0 TB/s,
 // with where the buffers lie), with 8-bit moments 10 (1.41 G: 14.1 GB in
-// 2.6 ms, 5.4 TB/s).  There the codes' arithmetic fills four fifths of the
-// VALU's time beside the accesses: some 50 operations an element, from 56
+// 2.55 to 2.7 ms, 5.2 to 5.5 TB/s).  There the codes' arithmetic fills four
+// fifths of the VALU's time beside the accesses: some 52 operations an element
 // (3.36 ms before the hardware's root and reciprocal, the exponent by lane
 // exchange and the once-a-block checks; without any of it the same accesses
 // take 2.56 ms).  Large blocks or several groups a thread for float32 moments
