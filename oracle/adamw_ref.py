@@ -1,4 +1,4 @@
-"""AdamW with moments in 32 or 8 bits, restated in numpy: the checker of rhp_adamw_step.
+"""AdamW with moments in 32 or 8 bits, restated in numpy: what rhp_adamw_step is tested against.
 
 ``update`` runs the step in one float type, operation by operation; with
 float32 it is what the kernel does, with float64 the mathematics.  ``weight``
