@@ -527,16 +527,20 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
         if constexpr (kAhead) load(nxt, t + stride);
         float c[2] = {0.0f, 0.0f};   // sums of g xh and of g
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            float gx = 0.0f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float d = cur.dy[v].at(j), xh = (cur.x[v].at(j) - cur.mu) * cur.r;
                 aw[v][j] += d * xh;
                 ab[v][j] += d;
                 const float g = at.counts(v, j) ? d * wv[v][j] : 0.0f;
-                c[0] += g * xh;
+                gx += g * xh;
                 c[1] += g;
             }
+            // A chunk past the row is zeros, but -mean * rstd can be infinite where no xh of the row is.
+            c[0] += at.on[v] ? gx : 0.0f;
+        }
         if (dx) {
             row_sums<2, TPR>(c, red[turn]);
             const float c1 = c[0] / static_cast<float>(h), c2 = c[1] / static_cast<float>(h);

@@ -223,6 +223,21 @@ def test_rows_that_are_constant_huge_or_not_finite(h):
     assert torch.isnan(dx[2:4]).all() and torch.isnan(dw).any() and torch.isfinite(db).all()
 
 
+@pytest.mark.parametrize("dt,h", [(torch.bfloat16, 8), (torch.bfloat16, 24), (torch.bfloat16, 100), (torch.float32, 4),
+                                  (torch.float32, 36), (torch.float32, 50)])
+def test_a_mean_whose_product_with_rstd_overflows(dt, h):
+    """Rows of 2^120 (their sums are exact): mean * rstd is past float32, the gradient is not."""
+    say(f"norm huge mean h={h} {dt}")
+    _, w, b, dy, dres = _inputs(5, h, dt, torch.float32, seed=h)
+    x = torch.full((5, h), 2.0 ** 120, dtype=dt)
+    dev = [t.to(DEV) for t in (x, w, b, dy, dres)]
+    y, mean, rstd = K.layer_norm(*dev[:3], 1e-5)
+    assert torch.equal(mean.cpu(), torch.full((5,), 2.0 ** 120)) and torch.equal(y.cpu(), b.to(dt).expand(5, h))
+    for res in (None, 4):
+        dx, dw, db = K.layer_norm_bwd(dev[3], dev[0], dev[1], mean, rstd, dres=None if res is None else dev[4])
+        _check_backward(dy, x, w, mean, rstd, None if res is None else dres, dx, dw, db, torch.float32)
+
+
 def test_offsets_past_two_gigabytes():
     """More than 2^31 elements: the last rows are what they are in a batch of their own."""
     T, h = (1 << 31) // 4096 + 40, 4096
