@@ -435,7 +435,7 @@ int rhp_adam_step(int count, void* const* params, const void* const* grads, void
  *   [T] float (double for F64 rows), what rhp_layer_norm_bwd takes.
  * Statistics are float: a row whose centred squares leave its range (values
  * past about 1e18) has rstd 0.
- * y must not overlap x.  Any 1 <= h <= 2^28, any T; rows need only their
+ * y must not overlap x.  Any 1 <= h <= 2^26, any T; rows need only their
  * element's alignment.  A row's results depend on that row alone, whatever T.
  */
 int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const void* b, int w_dtype, int64_t T, int h,

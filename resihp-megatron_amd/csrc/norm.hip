@@ -656,7 +656,7 @@ int check_norm(const char* what, int dtype, int w_dtype, int64_t T, int h) {
     RHP_REQUIRE(w_dtype == dtype || (dtype == RHP_BF16 && w_dtype == RHP_F32),
                 std::string(what) + ": weight and bias must have the rows' dtype (or float32 with bfloat16 rows)");
     RHP_REQUIRE(T >= 0, std::string(what) + ": negative row count");
-    RHP_REQUIRE(h >= 1 && h <= (1 << 28), std::string(what) + ": h must be between 1 and 2^28");
+    RHP_REQUIRE(h >= 1 && h <= (1 << 26), std::string(what) + ": h must be between 1 and 2^26");
     return 0;
 }
 

@@ -257,6 +257,17 @@ def test_offsets_past_two_gigabytes():
     assert ((db.double() - want).abs() <= (T // 16 + 600) * 2.0 ** -24 * T * 20).all()
 
 
+def test_the_longest_rows():
+    h = (1 << 26) - 3
+    say(f"norm h={h}")
+    x, w, b, dy, _ = _inputs(1, h, torch.bfloat16, torch.float32)
+    dev = [t.to(DEV) for t in (x, w, b, dy)]
+    y, mean, rstd = K.layer_norm(*dev[:3], 1e-5)
+    _check_forward(x, w, b, 1e-5, y, mean, rstd)
+    dx, dw, db = K.layer_norm_bwd(dev[3], dev[0], dev[1], mean, rstd)
+    _check_backward(dy, x, w, mean, rstd, None, dx, dw, db, torch.float32)
+
+
 def test_refusals():
     x = torch.zeros(4, 64, device=DEV, dtype=torch.bfloat16)
     w = torch.ones(64, device=DEV)

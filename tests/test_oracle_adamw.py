@@ -230,6 +230,18 @@ def test_layer_norm_bwd_refusals(kw, msg):
                a["dx"] or None, FAKE, FAKE, a["ws"], a["size"], None)
 
 
+def test_layer_norm_refuses_rows_past_its_launches():
+    """The partial rows are summed by 1024 threads for every 64 of their 2 h columns: at h = 2^27 that would be
+    2^32 threads, which no launch has."""
+    _norm_fwd(T=0, h=1 << 26)
+    for h in ((1 << 26) + 1, 1 << 27, 1 << 28):
+        with pytest.raises(RuntimeError, match="h must be"):
+            _norm_fwd(T=0, h=h)
+        with pytest.raises(RuntimeError, match="h must be"):
+            C.call("rhp_layer_norm_bwd", FAKE, FAKE, C.F32, FAKE, C.F32, FAKE, FAKE, None, 0, h, 2 * FAKE, None, None,
+                   None, 0, None)
+
+
 def test_workspace_queries():
     L = C.lib()
     assert L.rhp_layer_norm_bwd_workspace_bytes(-1, 64, C.F32) == 0 and L.rhp_layer_norm_bwd_workspace_bytes(4, 0, C.F32) == 0
