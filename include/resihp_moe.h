@@ -502,7 +502,8 @@ int rhp_adamw_plan(int count, void* const* params, const int* dtypes, void* cons
  * device float that every gradient is multiplied with (NULL: 1), read when the
  * step runs.  step counts from 1; betas in [0, 1), lr, eps and weight_decay not
  * negative.  The scalars are fixed when the call is
- * enqueued, in a captured graph too.  One launch for up to 448 tensors.
+ * enqueued, in a captured graph too.  One launch for up to 448 tensors and 2^30
+ * elements (2^32 with moments in 8 bits).
  */
 int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
                    const int* g_dtypes, double lr, double beta1, double beta2, double eps, double weight_decay,

@@ -61,6 +61,7 @@ constexpr int kGroups8 = 2, kElems8 = 8 * kGroups8, kElems32 = 4;   // elements 
 constexpr int kBlock8 = kThreads * kElems8, kBlock32 = kThreads * kElems32;
 constexpr int kScaleBlock = 128;       // elements that share an exponent
 constexpr int kMaxGrads = 448;         // tensors a launch takes (their gradients' pointers are kernel arguments)
+constexpr uint32_t kMaxBlocks = 1 << 20;   // blocks a launch takes: HIP has no launch of 2^32 threads
 
 // ------------------------------------------------------------------ the plan
 
@@ -611,9 +612,11 @@ int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grad
         Grads g{};
         for (uint32_t t = t0; t < t1; ++t)
             if (grads && grads[t]) g.g[t - t0] = tag(grads[t], g_dtypes[t]);
-        hipLaunchKernelGGL((adamw_kernel<A, kState8, kTinyEps>), dim3(b1 - b0), dim3(kThreads), 0, stream, tensors,
-                           of_block, g, t0, b0, s, grad_scale, salt);
-        if (int rc = check_launch("adamw_kernel")) return rc;
+        for (uint32_t b = b0; b < b1; b += kMaxBlocks) {
+            hipLaunchKernelGGL((adamw_kernel<A, kState8, kTinyEps>), dim3(std::min(b1 - b, kMaxBlocks)), dim3(kThreads),
+                               0, stream, tensors, of_block, g, t0, b, s, grad_scale, salt);
+            if (int rc = check_launch("adamw_kernel")) return rc;
+        }
     }
     return 0;
 }
@@ -627,7 +630,7 @@ extern "C" size_t rhp_adamw_plan_bytes(int count, const int64_t* numel, int stat
     if (count < 0 || (count > 0 && !numel) || (state_bits != 32 && state_bits != 8)) return 0;
     uint64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
-        if (numel[i] < 0) return 0;
+        if (numel[i] < 0 || numel[i] > (int64_t(1) << 34)) return 0;
         blocks += static_cast<uint64_t>(blocks_of(numel[i], state_bits == 8));
     }
     return plan_bytes(static_cast<uint64_t>(count), blocks);

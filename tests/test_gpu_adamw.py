@@ -328,6 +328,15 @@ def test_a_tensor_of_more_than_two_giga_elements(bits):
     assert abs(K.grad_norm([g])[0].item() - np.sqrt((hg.astype(np.float64) ** 2).sum())) < 1e-4
 
 
+def test_every_element_is_stepped_where_a_step_takes_several_launches():
+    n = (2 << 30) + 3001
+    say(f"adamw n={n} without a gradient")
+    p = torch.ones(n, dtype=torch.bfloat16, device=DEV)
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    K.adamw_step(K.AdamWPlan([p], [m], [v]), [None], 0.5, (0.9, 0.999), 1e-8, 1.0, 1)
+    assert all(bool((t == 0.5).all()) for t in p.split(1 << 28))
+
+
 def test_gradients_with_strides_and_parameters_twice():
     say("adamw strided gradient")
     a, b = (moe.AdamW({"w": torch.nn.Parameter(seeded((40, 70), 1, 0.05).to(DEV))}, **HYPER) for _ in range(2))

@@ -150,6 +150,12 @@ def test_plan_refuses_bad_counts():
                    C.ptr_array([FAKE]), None, (ctypes.c_int64 * 1)(n), None, None, 32, buf, 4096)
 
 
+def test_plan_bytes_of_counts_out_of_range():
+    for n in ((1 << 34) + 1, (1 << 63) - 1):
+        assert C.lib().rhp_adamw_plan_bytes(1, (ctypes.c_int64 * 1)(n), 32) == 0
+    assert C.lib().rhp_adamw_plan_bytes(1, (ctypes.c_int64 * 1)(1 << 34), 8) > 0
+
+
 def _step(image, size, grads=None, codes=None, step=1, dev=FAKE, hyper=(1e-3, 0.9, 0.999, 1e-8, 0.0)):
     C.call("rhp_adamw_step", image, dev, size, C.ptr_array(grads) if grads else None,
            (ctypes.c_int * 1)(*codes) if codes else None, *hyper, step, None, 0, None)
