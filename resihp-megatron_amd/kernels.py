@@ -877,7 +877,7 @@ class AdamWPlan:
                 _expect(masters[i].dtype == torch.float32 and masters[i].shape == p.shape,
                         f"master {i} must be float32 with the param's shape")
         self.params, self.tensors = list(params), (list(exp_avg), list(exp_avg_sq), scales, masters)
-        self.shapes = [p.shape for p in params]
+        self.shapes, self.strides = [p.shape for p in params], [p.stride() for p in params]
         self.dtypes = [p.dtype for p in params]
         self.ptrs = [p.data_ptr() for p in params]
         self.numel = numel = _host_array(ctypes.c_int64, [p.numel() for p in params])
@@ -892,19 +892,22 @@ class AdamWPlan:
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def moved(self) -> bool:
-        """Whether a parameter's storage is no longer where the plan has it."""
-        return list(map(_T.data_ptr, self.params)) != self.ptrs
+        """Whether a parameter is no longer where the plan has it, or no longer laid out so."""
+        ps = self.params
+        return (list(map(_T.data_ptr, ps)) != self.ptrs or list(map(_T.size, ps)) != self.shapes
+                or list(map(_T.stride, ps)) != self.strides)
 
 
 _GRAD_DT = {torch.float32: C.F32, torch.bfloat16: C.BF16}
 
 
 class PlanGrads:
-    """A plan's gradients, checked, with the arrays that the calls of one step take.  Not kept beyond it."""
+    """A plan's gradients, checked, with the arrays that the calls of one step take.  Not kept beyond it.
+    ``moved``: what plan.moved() has just said, where it was asked."""
 
-    def __init__(self, plan: AdamWPlan, grads):
+    def __init__(self, plan: AdamWPlan, grads, moved: bool | None = None):
         _expect(len(grads) == len(plan.params), "one gradient (or None) per parameter")
-        if plan.moved():
+        if plan.moved() if moved is None else moved:
             raise KernelArgumentError("a parameter's storage has moved since the AdamW plan was made")
         taken = {torch.float64: C.F64} if plan.dtypes[0] is torch.float64 else _GRAD_DT
         there = [g for g in grads if g is not None]

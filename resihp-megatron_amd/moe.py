@@ -364,9 +364,9 @@ class AdamW:
             self._plan = self._make_plan()
         plan = self._plan
         try:
-            grads = K.PlanGrads(plan, grads)
+            grads = K.PlanGrads(plan, grads, moved=False)
         except K.KernelArgumentError:   # gradients with strides, or what a copy does not mend
-            grads = K.PlanGrads(plan, [None if g is None else g.contiguous() for g in grads])
+            grads = K.PlanGrads(plan, [None if g is None else g.contiguous() for g in grads], moved=False)
         norm = K.grad_norm(grads, self.max_grad_norm) if self.max_grad_norm is not None and grads.any else None
         K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
                      None if norm is None else norm[1:], self.seed)

@@ -276,6 +276,25 @@ def test_parameters_that_move_are_followed():
         K.adamw_step(plan, [None, None], 1e-3, (0.9, 0.999), 1e-8, 0.0, 1)
 
 
+@pytest.mark.parametrize("anew", [lambda t: t.t(), lambda t: t[:32], lambda t: t.reshape(32, 128)],
+                         ids=["transposed", "fewer-rows", "reshaped"])
+def test_parameters_laid_out_anew_in_place_are_refused(anew):
+    """At the same address with another shape or other strides: the moments no longer belong to the elements."""
+    say("adamw parameter laid out anew")
+    p = torch.nn.Parameter(seeded((64, 64), 1).to(DEV))
+    opt = moe.AdamW({"p": p})
+    opt.step()
+    old = p.data
+    p.data = anew(old)
+    before = old.clone()
+    with pytest.raises(RuntimeError):
+        opt.step()
+    assert opt.step_count == 1 and torch.equal(old, before)
+    p.data = old
+    opt.step()
+    assert opt.step_count == 2 and not torch.equal(old, before)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("eps", [0.0, 1e-20, 1.9e-12, 2.1e-12, 1e-3])
 def test_eps_down_to_zero(bits, eps):
