@@ -929,7 +929,8 @@ class PlanGrads:
 
 def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
                step: int, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
-    """One AdamW step over the plan's tensors, in place, in one launch (up to 448 tensors).
+    """One AdamW step over the plan's tensors, in place, in one launch (up to 448 tensors and 2^30
+    elements, 2^32 with moments in 8 bits).
 
     ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights), or the plan's
     ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device that
