@@ -892,10 +892,10 @@ class AdamWPlan:
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def moved(self) -> bool:
-        """Whether a parameter is no longer where the plan has it, or no longer laid out so."""
+        """Whether a parameter is no longer where the plan has it, or no longer of that type or laid out so."""
         ps = self.params
         return (list(map(_T.data_ptr, ps)) != self.ptrs or list(map(_T.size, ps)) != self.shapes
-                or list(map(_T.stride, ps)) != self.strides)
+                or list(map(_T.stride, ps)) != self.strides or list(map(_T.dtype.__get__, ps)) != self.dtypes)
 
 
 _GRAD_DT = {torch.float32: C.F32, torch.bfloat16: C.BF16}

@@ -1,0 +1,51 @@
+"""What an AdamW optimizer holds beside its moments: which tensors its plan steps, which of its settings a step
+reads, which states it takes."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from _helpers import DEV, say, seeded
+from oracle import adamw_ref as R
+from resihp_megatron_amd import moe
+
+pytestmark = pytest.mark.gpu
+
+HYPER = dict(lr=2e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+def _param(n, seed, dtype=torch.float32):
+    return torch.nn.Parameter(seeded((n,), seed, 0.05).to(dtype).to(DEV))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_retyped_at_its_address_is_stepped_as_its_new_type(bits):
+    """float32 to bfloat16 over one buffer: the bytes behind the smaller tensor stay as they were."""
+    n = 3000
+    buf = torch.full((2 * n,), 7.0, device=DEV)
+    buf[:n] = seeded((n,), 1, 0.05).to(DEV)
+    p = torch.nn.Parameter(buf[:n])
+    opt = moe.AdamW({"p": p}, **HYPER, state_bits=bits)
+    p.grad = seeded((n,), 2).to(DEV)
+    say(f"adamw retyped parameter {bits}")
+    opt.step()
+    p.grad = None
+    p.data = buf.view(torch.bfloat16)[:n]
+    p.data.copy_(seeded((n,), 3, 0.05))
+    p.grad = seeded((n,), 4).to(torch.bfloat16).to(DEV)
+    behind, before = buf[n // 2:].clone(), p.detach().float().cpu().numpy().copy()
+    opt.step()
+    assert torch.equal(buf[n // 2:].view(torch.int32), behind.view(torch.int32))
+    m, v = (t.float().cpu().numpy()[:n] for t in opt.moments())
+    if bits == 32:      # (codes of 8 bits are what m and v became, not what the weight was stepped with)
+        want = R.weight(before, m, v, np.float64, *HYPER.values(), 2)
+        tol = 2.0 ** -24 * (4 * np.abs(before) + 16 * np.abs(want - before))
+        assert (np.abs(p.detach().double().cpu().numpy() - want) <= tol + 2.0 ** -8 * (np.abs(want) + tol)).all()
+    assert not torch.equal(p.detach().float().cpu(), torch.from_numpy(before))
+    p.grad = None
+    p.data = torch.zeros(n, dtype=torch.float64, device=DEV)
+    with pytest.raises(RuntimeError):
+        opt.step()
+    assert opt.step_count == 2
