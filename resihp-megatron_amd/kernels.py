@@ -12,6 +12,7 @@ from __future__ import annotations
 import array
 import collections
 import ctypes
+import operator
 
 from dataclasses import dataclass
 
@@ -890,6 +891,10 @@ class AdamWPlan:
                8 if eight else 32, self.image.data_ptr(), size)
         self.dev_image = self.image.to(self.device)
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def holds(self, params) -> bool:
+        """Whether these are the plan's parameters, in its order."""
+        return len(params) == len(self.params) and all(map(operator.is_, params, self.params))
 
     def moved(self) -> bool:
         """Whether a parameter is no longer where the plan has it, or no longer of that type or laid out so."""

@@ -319,11 +319,11 @@ class AdamW:
             raise ValueError("float64 parameters need an AdamW of their own, with 32-bit (here float64) moments")
         self._flat: dict[str, torch.Tensor] = {}
         self._plan: K.AdamWPlan | None = None
+        names = list(self.params)
+        self.state = {n: {} for n in names}
         if not self.params:
             return
-        names = list(self.params)
         state = torch.uint8 if state_bits == 8 else torch.float64 if f64 else torch.float32
-        self.state = {n: {} for n in names}
         for key in ("exp_avg", "exp_avg_sq"):
             self._allocate(key, names, state)
         if state_bits == 8:
@@ -360,7 +360,7 @@ class AdamW:
             self.step_count += 1
             return
         grads = [p.grad for p in self.params.values()]
-        if self._plan is None or self._plan.moved():
+        if self._plan is None or not self._plan.holds(self.params.values()) or self._plan.moved():
             self._plan = self._make_plan()
         plan = self._plan
         try:
@@ -377,6 +377,9 @@ class AdamW:
 
     def _make_plan(self) -> K.AdamWPlan:
         names = list(self.params)
+        strange = [n for n in names if n not in self.state]
+        if strange:
+            raise KeyError(f"AdamW has no state for the parameters {strange}")
         of = lambda key: [self.state[n].get(key) for n in names]  # noqa: E731
         return K.AdamWPlan([self.params[n] for n in names], of("exp_avg"), of("exp_avg_sq"),
                            of("scales") if self.state_bits == 8 else None, of("master"),

@@ -49,3 +49,22 @@ def test_a_parameter_retyped_at_its_address_is_stepped_as_its_new_type(bits):
     with pytest.raises(RuntimeError):
         opt.step()
     assert opt.step_count == 2
+
+
+def test_a_parameter_put_in_anothers_place_is_stepped():
+    """As Adam steps it: the optimizer's dict says whom the moments belong to, the plan follows."""
+    say("adamw replaced parameter")
+    a, b, other = _param(300, 1), _param(20, 2), _param(300, 1)
+    opt = moe.AdamW({"a": a, "b": b}, **HYPER)
+    for p in (a, b, other):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept = a.detach().clone()
+    other.data.copy_(a.data)
+    opt.params["a"] = other
+    opt.step()
+    assert torch.equal(a, kept) and not torch.equal(other, kept) and opt.step_count == 2
+    opt.params["new"] = _param(8, 3)
+    with pytest.raises(KeyError, match="new"):
+        opt.step()
+    assert opt.step_count == 2
