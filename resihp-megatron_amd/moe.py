@@ -288,7 +288,8 @@ class AdamW:
     rounded: ``seed``, the step and the parameter's name give the random bits, so a run is reproducible and
     a parameter keeps its own when it moves).  ``master_weights``: float32 masters of the bfloat16
     parameters, which are then the masters' rounded values.  ``max_grad_norm``: clips; ``grad_norm`` then
-    holds the last step's [norm, coefficient] on the device.  ``no_decay``: names without weight decay.
+    holds the last step's [norm, coefficient] on the device.  ``no_decay``: names without weight decay; like
+    ``lr`` and ``weight_decay``, what it is at a step counts.
 
     The state lives in a few flat buffers (``buffers()``), each tensor from a multiple of 128 elements on,
     in the order of ``params``; ``state_tensors()`` names views of it.
@@ -301,8 +302,6 @@ class AdamW:
             raise ValueError(f"the moments have 32 or 8 bits, not {state_bits}")
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError("max_grad_norm must be positive")
-        if any(n not in params for n in no_decay):
-            raise ValueError(f"no_decay names no parameter: {[n for n in no_decay if n not in params]}")
         for n, p in params.items():
             if not p.is_cuda:
                 raise RuntimeError(f"AdamW: parameter {n} is not on a HIP device; the fused step runs on the GPU")
@@ -321,6 +320,7 @@ class AdamW:
         self._plan: K.AdamWPlan | None = None
         names = list(self.params)
         self.state = {n: {} for n in names}
+        self._check_no_decay()
         if not self.params:
             return
         state = torch.uint8 if state_bits == 8 else torch.float64 if f64 else torch.float32
@@ -360,9 +360,11 @@ class AdamW:
             self.step_count += 1
             return
         grads = [p.grad for p in self.params.values()]
-        if self._plan is None or not self._plan.holds(self.params.values()) or self._plan.moved():
-            self._plan = self._make_plan()
         plan = self._plan
+        if (plan is None or set(self.no_decay) != self._plan_no_decay
+                or not plan.holds(self.params.values()) or plan.moved()):
+            plan = self._plan = self._make_plan()
+            self._plan_no_decay = set(self.no_decay)
         try:
             grads = K.PlanGrads(plan, grads, moved=False)
         except K.KernelArgumentError:   # gradients with strides, or what a copy does not mend
@@ -375,7 +377,13 @@ class AdamW:
         self.step_count += 1
         self.grad_norm = norm
 
+    def _check_no_decay(self) -> None:
+        unknown = [n for n in self.no_decay if n not in self.state]
+        if unknown:
+            raise ValueError(f"no_decay names no parameter: {unknown}")
+
     def _make_plan(self) -> K.AdamWPlan:
+        self._check_no_decay()
         names = list(self.params)
         strange = [n for n in names if n not in self.state]
         if strange:

@@ -68,3 +68,17 @@ def test_a_parameter_put_in_anothers_place_is_stepped():
     with pytest.raises(KeyError, match="new"):
         opt.step()
     assert opt.step_count == 2
+
+
+def test_no_decay_is_read_at_every_step():
+    say("adamw no_decay")
+    opt = moe.AdamW({"a": _param(300, 1), "b": _param(20, 2)}, lr=0.5, weight_decay=1.0)
+    for want in ((), ("a",), ("a", "b"), ("b",)):
+        opt.no_decay = set(want)
+        before = {n: p.detach().clone() for n, p in opt.params.items()}
+        opt.step()      # no gradients: only the decay moves a weight
+        for n, p in opt.params.items():
+            assert torch.equal(p, before[n] if n in want else before[n] * 0.5), (want, n)
+    opt.no_decay.add("c")
+    with pytest.raises(ValueError, match="no_decay"):
+        opt.step()
