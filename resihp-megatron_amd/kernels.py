@@ -891,6 +891,7 @@ class AdamWPlan:
                8 if eight else 32, self.image.data_ptr(), size)
         self.dev_image = self.image.to(self.device)
         self.stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        self.captured = False   # whether a graph has a step of it, which reads the image at every replay
 
     def holds(self, params) -> bool:
         """Whether these are the plan's parameters, in its order."""
@@ -940,7 +941,7 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights), or the plan's
     ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device that
     every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the random bits that round
-    moments of 8 bits."""
+    moments of 8 bits.  A graph that captures the step needs the plan for as long as it is replayed."""
     if not isinstance(grads, PlanGrads):
         grads = PlanGrads(plan, grads)
     if grads.plan is not plan:
@@ -948,8 +949,9 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     if grad_scale is not None:
         _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
                 "grad_scale must be one float32 on the plan's device")
-    if (torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream
-            and not torch.cuda.is_current_stream_capturing()):
+    if torch.cuda.is_current_stream_capturing():
+        plan.captured = True
+    elif torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream:
         # Should the plan be dropped while this step runs, its memory waits for this stream too.
         plan.dev_image.record_stream(torch.cuda.current_stream(plan.device))
     _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(),

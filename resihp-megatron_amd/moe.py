@@ -318,6 +318,7 @@ class AdamW:
             raise ValueError("float64 parameters need an AdamW of their own, with 32-bit (here float64) moments")
         self._flat: dict[str, torch.Tensor] = {}
         self._plan: K.AdamWPlan | None = None
+        self._captured: list[K.AdamWPlan] = []
         names = list(self.params)
         self.state = {n: {} for n in names}
         self._check_no_decay()
@@ -363,6 +364,8 @@ class AdamW:
         plan = self._plan
         if (plan is None or set(self.no_decay) != self._plan_no_decay
                 or not plan.holds(self.params.values()) or plan.moved()):
+            if plan is not None and plan.captured:
+                self._captured.append(plan)   # a graph reads its image at every replay
             plan = self._plan = self._make_plan()
             self._plan_no_decay = set(self.no_decay)
         try:

@@ -82,3 +82,43 @@ def test_no_decay_is_read_at_every_step():
     opt.no_decay.add("c")
     with pytest.raises(ValueError, match="no_decay"):
         opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_outlives_a_moved_parameter(bits):
+    """A captured step reads its plan's image at every replay: the optimizer keeps that plan when it makes another,
+    and the graph goes on stepping the storage that it was captured with."""
+    say(f"adamw graph after a move {bits}")
+    n = 3000
+    opt = moe.AdamW({"p": _param(n, 1), "q": _param(40, 2)}, **HYPER, state_bits=bits)
+    p = opt.params["p"]
+    for t in opt.params.values():
+        t.grad = torch.ones_like(t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        opt.step()
+    old, size = p.data, opt._plan.dev_image.numel()
+    p.data = old.clone()
+    opt.step()
+    torch.cuda.synchronize()
+    junk = [torch.full((size,), 0xAB, dtype=torch.uint8, device=DEV) for _ in range(64)]   # takes what was given back
+    held = [old, opt.params["q"].data, *(t for b in opt.state.values() for t in b.values())]
+    for _ in range(3):
+        saved, moved = [t.clone() for t in held], p.detach().clone()
+        gr.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert torch.equal(p.detach(), moved) and not torch.equal(got[0], saved[0])
+        for t, s in zip(held, saved):
+            t.copy_(s)
+        new, p.data, opt.step_count = p.data, old, 1
+        opt.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, held))
+        p.data = new
+    assert len(junk) == 64
