@@ -451,7 +451,8 @@ size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype);
  * dres ([T,h] dtype, or NULL) is the gradient that reaches x beside the norm
  * (the residual's).  dx may be NULL, dw and db ([h] w_dtype) too; what is NULL
  * is not computed.  T == 0 writes zeros to dw and db.  Sums are float (double
- * for F64 rows) in an order that the sizes fix.  Outputs must not overlap
+ * for F64 rows, and over the columns of rows past 32 KB) in an order that the
+ * sizes fix.  Outputs must not overlap
  * inputs.  The workspace (16-byte aligned) is only needed
  * with dw or db and holds nothing between calls.
  */

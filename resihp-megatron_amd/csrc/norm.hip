@@ -11,8 +11,9 @@
 //   dx   = rstd * (g - sum(g) / h - xh * sum(g * xh) / h) (+ the residual's gradient)
 //   dw   = sum over rows of dy * xh      db = sum over rows of dy
 //
-// Sums and statistics are float (double for double rows); a bfloat16 result
-// is rounded once, when it is stored.  The variance is that of the centred
+// Statistics are float (double for double rows) and so are sums, but those over
+// the columns of rows past the registers, which are double; a bfloat16 result is
+// rounded once, when it is stored.  The variance is that of the centred
 // values, so a large mean does not swamp it.  Nothing uses atomics: every sum
 // has an order fixed by the sizes, so results are reproducible bit for bit.
 //
@@ -107,18 +108,34 @@ template <int N, class W> __device__ __forceinline__ void load_again(const W* p,
 // caches.  For float64, and for rows that are too short or too long for
 // registers (below).  3355 rows of 20000 bfloat16: forward 78 us, 3.5 TB/s;
 // backward 164 us, which reads dy and x a second time for the columns' sums.
+//
+// A thread's share of a row has no bound but h / 256, so the sums B of rows
+// past the registers are double: the values of a chunk are added in pairs in
+// the rows' type (three additions at most), the chunks' sums in double, and one
+// rounding to float ends it.  (In float a row of 2^26 equal values had a mean
+// off by 0.25 %.)  Rows under a chunk, at most seven values, keep float sums:
+// 4 M rows of 5 bfloat16 forward 2.8 ms, with double ones 5.0, the exchange
+// between lanes being two words.
 
 // Sum of v over the block's threads, in every thread; `s` holds one value a
 // wave.  Ends with all threads past their reads of `s`.
-template <class A> __device__ __forceinline__ A block_sum(A v, A* s) {
+template <class B> __device__ __forceinline__ B block_sum(B v, B* s) {
     v = lane_sum<64>(v);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
-    A t = s[0];
+    B t = s[0];
 #pragma unroll
     for (int i = 1; i < kNormWaves; ++i) t += s[i];
     __syncthreads();
     return t;
+}
+// The sum of a piece's values, added in pairs (v is used up).
+template <int N, class A> __device__ __forceinline__ A pair_sum(A (&v)[N]) {
+#pragma unroll
+    for (int d = 1; d < N; d *= 2)
+#pragma unroll
+        for (int j = 0; j < N; j += 2 * d) v[j] += v[j + d];
+    return v[0];
 }
 
 // Calls f(first, count) for the thread's pieces of a row: whole chunks, then single elements of the rest.
@@ -134,33 +151,33 @@ template <int N, class S> __device__ __forceinline__ void piece(const S* p, int 
         load_again<N>(p + i, v);
 }
 
-template <class S, class W>
+template <class B, class S, class W>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const S* __restrict__ x, const W* __restrict__ w,
                                                                 const W* __restrict__ b, int64_t T, int h,
                                                                 typename Elem<S>::acc eps, S* __restrict__ y,
                                                                 typename Elem<S>::acc* __restrict__ mean,
                                                                 typename Elem<S>::acc* __restrict__ rstd) {
     using A = typename Elem<S>::acc;
-    __shared__ A s[kNormWaves];
+    __shared__ B s[kNormWaves];
     for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
         const S* row = x + t * h;
-        A sum = 0, sq = 0;
+        B sum = 0, sq = 0;
+        for_pieces<kVec<S>>(h, [&](int i, auto n) {
+            constexpr int N = decltype(n)::value;
+            A v[N];
+            piece<N>(row, i, v);
+            sum += pair_sum<N>(v);
+        });
+        const A mu = static_cast<A>(block_sum(sum, s) / B(h));
         for_pieces<kVec<S>>(h, [&](int i, auto n) {
             constexpr int N = decltype(n)::value;
             A v[N];
             piece<N>(row, i, v);
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum += v[j];
+            for (int j = 0; j < N; ++j) v[j] = (v[j] - mu) * (v[j] - mu);
+            sq += pair_sum<N>(v);
         });
-        const A mu = block_sum(sum, s) / A(h);
-        for_pieces<kVec<S>>(h, [&](int i, auto n) {
-            constexpr int N = decltype(n)::value;
-            A v[N];
-            piece<N>(row, i, v);
-#pragma unroll
-            for (int j = 0; j < N; ++j) sq += (v[j] - mu) * (v[j] - mu);
-        });
-        const A r = rsqrt_t(block_sum(sq, s) / A(h) + eps);
+        const A r = rsqrt_t(static_cast<A>(block_sum(sq, s) / B(h)) + eps);
         for_pieces<kVec<S>>(h, [&](int i, auto n) {
             constexpr int N = decltype(n)::value;
             A v[N], wv[N], bv[N];
@@ -186,17 +203,17 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(const S* __restr
 }
 
 // The input gradient.
-template <class S, class W>
+template <class B, class S, class W>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const W* __restrict__ w,
     const typename Elem<S>::acc* __restrict__ mean, const typename Elem<S>::acc* __restrict__ rstd,
     const S* __restrict__ dres, int64_t T, int h, S* __restrict__ dx) {
     using A = typename Elem<S>::acc;
-    __shared__ A s[kNormWaves];
+    __shared__ B s[kNormWaves];
     for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
         const A mu = mean[t], r = rstd[t];
         const S *xr = x + t * h, *gr = dy + t * h;
-        A c1 = 0, c2 = 0;
+        B s1 = 0, s2 = 0;
         const auto load = [&](int i, auto n, A* g, A* xh) {
             constexpr int N = decltype(n)::value;
             A wv[N];
@@ -214,13 +231,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(
             A g[N], xh[N];
             load(i, n, g, xh);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                c1 += g[j] * xh[j];
-                c2 += g[j];
-            }
+            for (int j = 0; j < N; ++j) xh[j] *= g[j];
+            s1 += pair_sum<N>(xh);
+            s2 += pair_sum<N>(g);
         });
-        c1 = block_sum(c1, s) / A(h);
-        c2 = block_sum(c2, s) / A(h);
+        const A c1 = static_cast<A>(block_sum(s1, s) / B(h)), c2 = static_cast<A>(block_sum(s2, s) / B(h));
         for_pieces<kVec<S>>(h, [&](int i, auto n) {
             constexpr int N = decltype(n)::value;
             A g[N], xh[N], v[N];
@@ -695,6 +710,12 @@ template <class F> int with_row_shape(RowShape r, F f) {
     }
 }
 
+// f(a zero of the type that the any-length kernels sum in): the rows' own for short rows, else double.
+template <class A, class F> int with_sums(bool few, F f) {
+    if (few) return f(A(0));
+    return f(0.0);
+}
+
 // f(whether rows end inside a chunk); rows of four chunks a thread do not (row_shape).
 template <int NV, class F> int with_tail(bool tail, F f) {
     if constexpr (NV < 4)
@@ -726,9 +747,11 @@ int norm_fwd(const void* x, const void* w, const void* b, int64_t T, int h, doub
         const RowShape shape = row_shape(sizeof(S) == 4 ? RHP_F32 : RHP_BF16, h, false);
         if (shape.tpr) return with_row_shape(shape, launch);
     }
-    hipLaunchKernelGGL((norm_fwd_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp, wp, bp, T, h,
-                       static_cast<A>(eps), yp, mp, rp);
-    return check_launch("norm_fwd_kernel");
+    return with_sums<A>(h < kVec<S>, [&](auto b) {
+        hipLaunchKernelGGL((norm_fwd_kernel<decltype(b), S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, xp,
+                           wp, bp, T, h, static_cast<A>(eps), yp, mp, rp);
+        return check_launch("norm_fwd_kernel");
+    });
 }
 
 template <class S, class W>
@@ -766,9 +789,12 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
         if (shape.tpr) return with_row_shape(shape, launch);
     }
     if (dx) {
-        hipLaunchKernelGGL((norm_bwd_rows_kernel<S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0, stream, dyp, xp, wp,
-                           mp, rp, resp, T, h, dxp);
-        if (int rc = check_launch("norm_bwd_rows_kernel")) return rc;
+        const int rc = with_sums<A>(h < kVec<S>, [&](auto b) {
+            hipLaunchKernelGGL((norm_bwd_rows_kernel<decltype(b), S, W>), dim3(row_grid(T)), dim3(kNormThreads), 0,
+                               stream, dyp, xp, wp, mp, rp, resp, T, h, dxp);
+            return check_launch("norm_bwd_rows_kernel");
+        });
+        if (rc) return rc;
     }
     if (!sums) return 0;
     const int slices = norm_slices(T, h);

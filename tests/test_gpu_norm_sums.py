@@ -1,0 +1,75 @@
+"""Layer norm's sums on the GPU where they are long: over the columns of rows past the registers, over many rows."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from _helpers import DEV, say
+from resihp_megatron_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+LONG = [(torch.bfloat16, h) for h in (16392, 20001, (1 << 20) + 3, 1 << 24, (1 << 26) - 3, 1 << 26)] + \
+       [(torch.float32, h) for h in (8196, 20001, (1 << 20) + 3, (1 << 24) + 1, 1 << 26)]
+
+
+def _close(got, want, tol, what):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((got.double() - want).abs()[bad].max()))
+
+
+@pytest.mark.parametrize("dt,h", LONG)
+def test_a_long_constant_row_gives_the_bias(dt, h):
+    say(f"norm constant h={h} {dt}")
+    x = torch.full((2, h), 0.1, device=DEV).to(dt)
+    x[1] = -7.3
+    b = torch.full((h,), 0.25, device=DEV)
+    y, mean, rstd = K.layer_norm(x, None, b, 1e-5)
+    assert torch.equal(mean, x[:, 0].float())
+    assert torch.equal(y, torch.full_like(y, 0.25))
+    assert ((rstd.double() - 1e-5 ** -0.5).abs() <= 4 * U * 1e-5 ** -0.5).all()
+
+
+@pytest.mark.parametrize("dt,h", LONG)
+def test_long_rows_against_float64(dt, h):
+    """Sums that no length dims: D additions in float (a chunk of at most eight values in pairs), the rest in double.
+    Every element's part is seen: the rows are zeros but for a few large ones, in the last chunk and behind it."""
+    D = 4
+    g = torch.Generator(device=DEV).manual_seed(h)
+    for at in (None, h - 1, h // 8 * 8 - 1, 0, 5000):
+        say(f"norm h={h} {dt} at={at}")
+        if at is None:
+            x = (torch.rand(1, h, generator=g, device=DEV) + 0.5).to(dt)      # one sign: no errors cancel
+        else:
+            x = torch.zeros(1, h, device=DEV, dtype=dt)
+            x[0, at] = 1024.0
+        y, mean, rstd = K.layer_norm(x, None, None, 1e-5)
+        xd = x.double()
+        m = xd.mean(1, keepdim=True)
+        c = xd - m
+        var = (c * c).mean(1, keepdim=True)
+        r = (var + 1e-5).rsqrt()
+        em = (D + 2) * U * xd.abs().mean(1, keepdim=True)
+        ev = (D + 4) * U * var + em * em + 2 * U * (c.abs() * xd.abs()).mean(1, keepdim=True)
+        er = r * (0.5 * ev / (var + 1e-5) + 4 * U)
+        _close(mean, m[:, 0], em[:, 0], "mean")
+        _close(rstd, r[:, 0], er[:, 0], "rstd")
+        want = c * r
+        tol = r * (em + U * c.abs()) + c.abs() * er + 2 * U * c.abs() * r
+        _close(y, want, tol * 1.01 + (want.abs() + tol) * torch.finfo(dt).eps / 2, "y")
+        del y, c, want, tol
+        # Backward: the same for the sums of g and of g xh, whose terms have roundings of their own.
+        dy = (torch.rand(1, h, generator=g, device=DEV) + 0.5).to(dt)
+        dx, dw, db = K.layer_norm_bwd(dy, x, None, mean, rstd)
+        md, rd, dyd = mean.double()[:, None], rstd.double()[:, None], dy.double()
+        xh = (xd - md) * rd
+        c1, a1 = (dyd * xh).mean(1, keepdim=True), (dyd * xh).abs().mean(1, keepdim=True)
+        c2 = dyd.mean(1, keepdim=True)
+        want = rd * (dyd - c2 - xh * c1)
+        tol = rd * U * (3 * dyd + (D + 4) * c2 + xh.abs() * ((D + 8) * a1 + 6 * c1.abs()) + 4 * c2)
+        _close(dx, want, tol * 1.01 + (want.abs() + tol) * torch.finfo(dt).eps / 2, "dx")
+        wt = (dyd * xh)[0]
+        _close(dw, wt, 4 * U * wt.abs() * 1.01 + wt.abs() * torch.finfo(dt).eps / 2, "dw")
+        assert torch.equal(db, dy[0])
