@@ -255,7 +255,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(
 }
 
 // Partial sums of dw and db over a slice of the rows, a chunk of columns a lane: part[slice][0 | 1][h].  The
-// columns behind the last whole chunk go to the single lanes of the last block.
+// columns behind the last whole chunk go to the single lanes of the last block.  Of rows past the registers a lane
+// takes at most some 512 (norm_slices), one float sum; of shorter rows, single elements, T / 1024 and more: 64
+// at a time in float, these sums in double (16 K values of 0.1 one after the other in float are off by 1.5e-4).
+// Doubles for whole chunks took 45 -> 103 us.
 template <class S>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_cols_kernel(
     const S* __restrict__ dy, const S* __restrict__ x, const typename Elem<S>::acc* __restrict__ mean,
@@ -271,21 +274,31 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_cols_kernel(
     A* p = part + static_cast<int64_t>(blockIdx.y) * 2 * h;
     const auto add = [&](int col, auto n) {
         constexpr int M = decltype(n)::value;
-        A dw[M] = {}, db[M] = {};
-        for (int64_t t = t0 + wave; t < t1; t += kNormWaves) {
-            A g[M], v[M];
-            piece<M>(dy + t * h, col, g);
-            piece<M>(x + t * h, col, v);
+        using B = typename std::conditional<M == 1, double, A>::type;
+        B dw[M] = {}, db[M] = {};
+        for (int64_t t = t0 + wave; t < t1;) {
+            const int64_t end = M == 1 ? min(t1, t + 64 * kNormWaves) : t1;
+            A pw[M] = {}, pb[M] = {};
+            for (; t < end; t += kNormWaves) {
+                A g[M], v[M];
+                piece<M>(dy + t * h, col, g);
+                piece<M>(x + t * h, col, v);
+#pragma unroll
+                for (int j = 0; j < M; ++j) {
+                    pw[j] += g[j] * ((v[j] - mean[t]) * rstd[t]);
+                    pb[j] += g[j];
+                }
+            }
 #pragma unroll
             for (int j = 0; j < M; ++j) {
-                dw[j] += g[j] * ((v[j] - mean[t]) * rstd[t]);
-                db[j] += g[j];
+                dw[j] += pw[j];
+                db[j] += pb[j];
             }
         }
 #pragma unroll
         for (int j = 0; j < M; ++j) {
-            sums[wave][j][lane] = dw[j];
-            sums[wave][N + j][lane] = db[j];
+            sums[wave][j][lane] = static_cast<A>(dw[j]);
+            sums[wave][N + j][lane] = static_cast<A>(db[j]);
         }
     };
     const bool chunk = c < whole, single = !chunk && c - whole < h % N;
@@ -651,10 +664,14 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
 }
 
 constexpr int kNormMaxSlices = 256;
-inline int norm_slices(int64_t T, int h) {
+constexpr int kNormSliceRows = 2048;   // at most, where a lane's sums are float: 512 rows a lane
+inline int norm_slices(int64_t T, int h, int dtype) {
     // About eight blocks a CU of float64's chunks.
     const int64_t want = std::max<int64_t>(1, 2048 / ((h + 127) / 128));
-    return static_cast<int>(std::max<int64_t>(1, std::min({want, (T + 15) / 16, int64_t(kNormMaxSlices)})));
+    const int64_t slices = std::max<int64_t>(1, std::min({want, (T + 15) / 16, int64_t(kNormMaxSlices)}));
+    const bool in_double = dtype == RHP_F64 || h * static_cast<int64_t>(dtype_bytes(dtype)) < 16;
+    const int64_t least = in_double ? 1 : (T + kNormSliceRows - 1) / kNormSliceRows;
+    return static_cast<int>(std::max(slices, std::min<int64_t>(least, 65535)));
 }
 
 inline unsigned row_grid(int64_t T) { return static_cast<unsigned>(std::min<int64_t>(T, 1 << 20)); }
@@ -797,7 +814,7 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
         if (rc) return rc;
     }
     if (!sums) return 0;
-    const int slices = norm_slices(T, h);
+    const int slices = norm_slices(T, h, sizeof(S) == 8 ? RHP_F64 : sizeof(S) == 4 ? RHP_F32 : RHP_BF16);
     hipLaunchKernelGGL(norm_bwd_cols_kernel<S>, dim3(col_blocks(h, kVec<S>), slices), dim3(kNormThreads), 0, stream, dyp,
                        xp, mp, rp, T, h, slices, part);
     if (int rc = check_launch("norm_bwd_cols_kernel")) return rc;
@@ -829,7 +846,7 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
     if (T < 0 || h <= 0) return 0;
     const int64_t parts = row_shape(dtype, h, false).tpr ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
-                                                : norm_slices(T, h);
+                                                : norm_slices(T, h, dtype);
     return static_cast<size_t>(parts) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
 }
 

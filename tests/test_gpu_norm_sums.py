@@ -73,3 +73,23 @@ def test_long_rows_against_float64(dt, h):
         wt = (dyd * xh)[0]
         _close(dw, wt, 4 * U * wt.abs() * 1.01 + wt.abs() * torch.finfo(dt).eps / 2, "dw")
         assert torch.equal(db, dy[0])
+
+
+@pytest.mark.parametrize("dt,h,T,lane", [(torch.bfloat16, 5, (1 << 24) + 77, 64), (torch.float32, 3, (1 << 24) + 77, 64),
+                                         (torch.bfloat16, 20001, 3000, 58), (torch.bfloat16, 16392, 40000, 500)])
+def test_column_sums_of_many_rows_outside_the_registers(dt, h, T, lane):
+    """A lane's rows are summed in double, 64 in float at a time (rows under a chunk), or few are (at most 512): that
+    makes ``lane`` additions.  Beside them
+    there are the rounding of the lane's sum to float, three additions over the block's waves, and of at most 256
+    slices on 16 waves 15 + 15 additions, and the result's rounding."""
+    say(f"norm columns T={T} h={h} {dt}")
+    x = torch.full((T, h), 1.0, dtype=dt, device=DEV)
+    x[:, 1] = 3.0
+    dy = torch.full((T, h), 0.1, device=DEV).to(dt)
+    w = torch.ones(h, device=DEV, dtype=torch.float32)
+    mean, rstd = torch.full((T,), 0.5, device=DEV), torch.full((T,), 0.3, device=DEV)
+    _, dw, db = K.layer_norm_bwd(dy, x, w, mean, rstd, need_x=False)
+    want_b = T * dy[0].double()
+    want_w = (dy[0].double() * (x[0].double() - 0.5) * rstd[0].double()) * T
+    _close(db, want_b, (36 + lane) * U * want_b.abs(), "db")
+    _close(dw, want_w, (39 + lane) * U * want_w.abs(), "dw")      # each term: the centred value, xh and the product
