@@ -494,12 +494,20 @@ __global__ __launch_bounds__(fwd_threads(TPR)) void norm_fwd_reg_kernel(const S*
     }
 }
 
-constexpr int kNormMaxParts = 256;   // partial sums of dw and db (blocks of the backward): one a CU
+constexpr int kNormParts = 256;      // partial sums of dw and db (blocks of the backward): one a CU
+constexpr int kNormTurns = 512;      // rows a group sums in float, one after the other; past them there are more blocks
 
 // Up to so many turns one block takes all rows and writes dw and db itself, without the second launch: 4096-wide
 // bfloat16, 4 rows (two turns) 12.4 us a call and 24.0 waited for, against 15.2 and 25.1 in two blocks; 8 rows
 // (four turns) 11.9 and 26.5 against 15.2 and 25.4.
 constexpr int kOneBlockTurns = 2;
+// Blocks of the backward.
+inline int64_t bwd_blocks(int64_t T, int tpr) {
+    const int groups = bwd_threads(tpr) / tpr;
+    const int64_t turns = (T + groups - 1) / groups;
+    if (turns <= kOneBlockTurns) return 1;
+    return std::min(turns, std::max<int64_t>(kNormParts, (turns + kNormTurns - 1) / kNormTurns));
+}
 
 template <class S, int NV> struct BwdRow {
     Chunk<S> x[NV], dy[NV], res[NV];
@@ -790,9 +798,8 @@ int norm_bwd(const void* dy, const void* x, const void* w, const void* mean, con
     if (T == 0) return sums ? reduce(0) : 0;
     if constexpr (sizeof(S) < 8) {
         auto launch = [&](auto tpr, auto chunks) {
-            constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = bwd_threads(TPR), G = B / TPR;
-            const int64_t turns = (T + G - 1) / G;
-            const int64_t nb = turns <= kOneBlockTurns ? 1 : std::min<int64_t>(turns, kNormMaxParts);
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(chunks)::value, B = bwd_threads(TPR);
+            const int64_t nb = bwd_blocks(T, TPR);
             const auto go = [&](auto tl) {
                 hipLaunchKernelGGL((norm_bwd_reg_kernel<S, W, TPR, NV, decltype(tl)::value>),
                                    dim3(static_cast<unsigned>(nb)), dim3(B), 0, stream, dyp, xp, wp, mp, rp, resp, T, h,
@@ -845,8 +852,11 @@ extern "C" int rhp_layer_norm_fwd(const void* x, int dtype, const void* w, const
 
 extern "C" size_t rhp_layer_norm_bwd_workspace_bytes(int64_t T, int h, int dtype) {
     if (T < 0 || h <= 0) return 0;
-    const int64_t parts = row_shape(dtype, h, false).tpr ? std::min<int64_t>(std::max<int64_t>(T, 1), kNormMaxParts)
-                                                : norm_slices(T, h, dtype);
+    int64_t parts = 0;   // with or without a residual's gradient
+    for (const bool four : {false, true}) {
+        const int tpr = row_shape(dtype, h, four).tpr;
+        parts = std::max<int64_t>(parts, tpr ? bwd_blocks(T, tpr) : norm_slices(T, h, dtype));
+    }
     return static_cast<size_t>(parts) * 2 * h * (dtype == RHP_F64 ? 8 : 4);
 }
 

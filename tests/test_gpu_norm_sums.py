@@ -93,3 +93,19 @@ def test_column_sums_of_many_rows_outside_the_registers(dt, h, T, lane):
     want_w = (dy[0].double() * (x[0].double() - 0.5) * rstd[0].double()) * T
     _close(db, want_b, (36 + lane) * U * want_b.abs(), "db")
     _close(dw, want_w, (39 + lane) * U * want_w.abs(), "dw")      # each term: the centred value, xh and the product
+
+
+@pytest.mark.parametrize("T,h", [(1 << 28, 4), (300_000, 8188)])
+def test_column_sums_of_very_many_rows(T, h):
+    """A group of lanes adds at most 512 rows in float; then there are 3 additions between groups of a wave, at most 4
+    between a block's parts, the partial rows on 16 waves (T / 64 / 512 / 16 for the short rows) and 15 more, and the
+    roundings of a term (3) and of the result."""
+    say(f"norm columns T={T} h={h}")
+    x, dy = torch.full((T, h), 1.0, device=DEV), torch.full((T, h), 0.1, device=DEV)
+    mean, rstd = torch.full((T,), 0.5, device=DEV), torch.full((T,), 0.3, device=DEV)
+    _, dw, db = K.layer_norm_bwd(dy, x, None, mean, rstd, need_x=False)
+    tol = (512 + 3 + 4 + max(37, -(-T // (64 * 512 * 16))) + 15 + 4) * U
+    want_b = T * dy[0].double()
+    want_w = (dy[0].double() * 0.5 * rstd[0].double()) * T
+    _close(db, want_b, tol * want_b.abs(), "db")
+    _close(dw, want_w, tol * want_w.abs(), "dw")
