@@ -351,8 +351,9 @@ constexpr int kDtypeShift = 60;
 
 // sqrt(v) and m / d.  In float by the hardware's square root and reciprocal (each within one unit in the last
 // place; the update is rounded once more into a weight some hundred times its size).  They may take subnormals
-// for zero: a subnormal v has a root under 1.1e-19, which beside eps >= 2e-12 is less than half a unit of d.
-// With a smaller eps (kTinyEps) the correctly rounded forms run.
+// for zero: a subnormal v has a root under 1.1e-19, and times ibc2s, which is 1000 at the first step of b2 =
+// 1 - 1e-6, it is less than half a unit of d beside eps >= 2e-12 ibc2s.  With a smaller eps (kTinyEps) the
+// correctly rounded forms run.
 template <bool kTinyEps> __device__ __forceinline__ float sqrt_of(float x) {
     return kTinyEps ? __builtin_sqrtf(x) : __builtin_amdgcn_sqrtf(x);
 }
@@ -361,7 +362,7 @@ template <bool kTinyEps> __device__ __forceinline__ float quotient(float m, floa
     return kTinyEps ? m / d : m * __builtin_amdgcn_rcpf(d);
 }
 template <bool kTinyEps> __device__ __forceinline__ double quotient(double m, double d) { return m / d; }
-constexpr double kLeastFastEps = 2e-12;
+constexpr double kLeastFastEps = 2e-12;   // times ibc2s
 __device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return a * b + c; }
 
@@ -747,7 +748,7 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
     const Scalars<float> f{static_cast<float>(d.b1), static_cast<float>(d.c1), static_cast<float>(d.b2),
                            static_cast<float>(d.c2), static_cast<float>(d.ibc2s), static_cast<float>(d.eps),
                            static_cast<float>(d.a), static_cast<float>(d.keep)};
-    if (eps < kLeastFastEps)
+    if (eps < kLeastFastEps * ibc2s)
         return head.state8 ? go(launch_step<float, true, true>, f) : go(launch_step<float, false, true>, f);
     return head.state8 ? go(launch_step<float, true, false>, f) : go(launch_step<float, false, false>, f);
 }

@@ -9,6 +9,7 @@ import torch
 
 from _helpers import DEV, say, seeded
 from oracle import adamw_ref as R
+from resihp_megatron_amd import kernels as K
 from resihp_megatron_amd import moe
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +123,28 @@ def test_a_graph_outlives_a_moved_parameter(bits):
         assert all(torch.equal(a, b) for a, b in zip(got, held))
         p.data = new
     assert len(junk) == 64
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("b2", [0.999, 0.999999])
+def test_small_second_moments_under_a_large_bias_correction(bits, b2):
+    """At the first steps the root is multiplied by up to 1 / sqrt(1 - b2) before eps is added: a subnormal second
+    moment shows beside an eps that hides it without that factor.  The weights are zeros, so that the update's 16 u
+    are all of the bound."""
+    n = 4096
+    for eps in (2.1e-12, 1e-10, 1e-8):
+        hyper = dict(lr=1.0, betas=(0.9, b2), eps=eps, weight_decay=0.0)
+        g32 = (seeded((n,), 2) * 10.0 ** torch.linspace(-21, -12, n))
+        p = torch.zeros(n, device=DEV)
+        sdt = torch.uint8 if bits == 8 else torch.float32
+        m, v = torch.zeros(n, dtype=sdt, device=DEV), torch.zeros(n, dtype=sdt, device=DEV)
+        sc = [torch.zeros(n // 128, 2, dtype=torch.uint8, device=DEV)] if bits == 8 else None
+        plan = K.AdamWPlan([p], [m], [v], sc, keys=[1])
+        say(f"adamw eps={eps} b2={b2} {bits}")
+        K.adamw_step(plan, [g32.to(DEV)], *hyper.values(), 1)
+        _, m32, v32 = R.update(np.zeros(n), g32.numpy(), np.zeros(n), np.zeros(n), np.float32, *hyper.values(), 1)
+        want = R.weight(np.zeros(n), m32, v32, np.float64, *hyper.values(), 1)
+        # m / d and a * it may be subnormal themselves: half of the smallest step each, times a at most.
+        tol = 2.0 ** -24 * 16 * np.abs(want) + 2.0 ** -149 * 16
+        bad = ~(np.abs(p.cpu().double().numpy() - want) <= tol)
+        assert not bad.any(), (int(bad.sum()), float((np.abs(p.cpu().double().numpy() - want) / np.abs(want))[bad].max()))
