@@ -513,6 +513,7 @@ int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes,
 /*
  * The values that n codes stand for, as bfloat16 (which holds each exactly),
  * and the codes nearest to n float moments.  scales: [ceil(n/128)][2] bytes.
+ * A v below zero makes its block NaN.
  */
 int rhp_moments_decode(const uint8_t* q_m, const uint8_t* q_v, const uint8_t* scales, int64_t n, void* m, void* v,
                        hipStream_t stream);

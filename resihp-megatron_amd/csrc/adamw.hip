@@ -307,7 +307,7 @@ __device__ __forceinline__ void encode_group(const float* m, const float* v, Ran
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         tm = max(tm, __float_as_uint(m[i]) & 0x7FFFFFFFu);
-        tv = max(tv, __float_as_uint(v[i]));   // a v with a sign is a NaN
+        tv = max(tv, __float_as_uint(v[i]));   // a v with a sign is a NaN (of -0 the callers make 0)
     }
     const uint32_t em = exponent_of(max16(tm)), ev = exponent_of(max16(tv) & 0x7FFFFFFFu);
     const int bm = base_of(em, 16), bv = base_of(ev, 32);
@@ -506,6 +506,9 @@ __global__ __launch_bounds__(kThreads) void moments_encode_kernel(const float* _
     float a[8], b[8];
     load_n<8>(m, e0, n, a);
     load_n<8>(v, e0, n, b);
+    // A caller's v, which a step's own cannot be: -0 is 0, and what has no root makes its block NaN as a NaN does.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = b[i] < 0.0f ? __builtin_nanf("") : __builtin_fabsf(b[i]);
     encode_group(a, b, [](int) { return 0x80008000u; }, e0, n, qm, qv, scales);
 }
 

@@ -979,7 +979,7 @@ def moments_decode(q_m: torch.Tensor, q_v: torch.Tensor, scales: torch.Tensor) -
 
 def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: torch.Tensor,
                    scales: torch.Tensor) -> None:
-    """Writes the 8-bit codes nearest to float32 moments."""
+    """Writes the 8-bit codes nearest to float32 moments; a v below zero makes its block of 128 NaN."""
     dev = _need_cuda(m, v, q_m, q_v, scales)
     n = _check_moments(q_m, q_v, scales)
     _expect(m.dtype == v.dtype == torch.float32 and m.numel() == v.numel() == n,

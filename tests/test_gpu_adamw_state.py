@@ -148,3 +148,30 @@ def test_small_second_moments_under_a_large_bias_correction(bits, b2):
         tol = 2.0 ** -24 * 16 * np.abs(want) + 2.0 ** -149 * 16
         bad = ~(np.abs(p.cpu().double().numpy() - want) <= tol)
         assert not bad.any(), (int(bad.sum()), float((np.abs(p.cpu().double().numpy() - want) / np.abs(want))[bad].max()))
+
+
+def test_negative_and_negative_zero_second_moments():
+    """-0 is a zero and leaves its block alone; a negative second moment has no root: its block reads as NaN."""
+    say("moments encode signs")
+    g = np.random.default_rng(5)
+    n = 128 * 5 + 40
+    m = g.standard_normal(n).astype(np.float32)
+    v = (g.standard_normal(n) ** 2).astype(np.float32)
+    v[[3, 128 * 2 + 5, n - 1]] = 0.0
+    plain = v.copy()
+    v[[3, 128 * 2 + 5, n - 1]] = -0.0
+    v[128 + 7] = -1e-6
+    v[128 * 3 + 100] = -np.inf
+    out = [torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV),
+           torch.zeros(6, 2, dtype=torch.uint8, device=DEV)]
+    K.moments_encode(torch.from_numpy(m).to(DEV), torch.from_numpy(v).to(DEV), *out)
+    want = R.encode(m, plain, R.nearest(n))
+    for b in (1, 3):
+        want[1][128 * b:128 * (b + 1)] = 0
+        want[2][b, 1] = 255
+    for t, e in zip(out, want):
+        assert np.array_equal(t.cpu().numpy(), e)
+    got = K.moments_decode(*out)[1].float().cpu().numpy().reshape(-1)
+    bad = np.zeros(n, bool)
+    bad[128:256] = bad[384:512] = True
+    assert np.array_equal(np.isnan(got), bad)
