@@ -415,30 +415,49 @@ class AdamW:
                 out[f"{key}/{n}"] = t
         return out
 
+    def _fitting(self, tensors: dict[str, torch.Tensor], n: str) -> tuple[torch.Tensor | None, ...]:
+        """The state of parameter ``n`` among ``tensors``: (param, exp_avg, exp_avg_sq, scales, master), the last
+        two None where there are none.  KeyError for what lacks, ValueError for what does not fit."""
+        p, m, v, sc, master = (tensors.get(f"{key}/{n}") for key in ("param", "exp_avg", "exp_avg_sq", "scales", "master"))
+        if p is None or n not in self.state:
+            raise KeyError(f"param/{n}")
+        if m is None or v is None or (torch.uint8 in (m.dtype, v.dtype) and sc is None):
+            raise KeyError(f"the moments of {n} are not all there")
+        shape = self.params[n].shape
+        eight = m.dtype == v.dtype == torch.uint8
+        for what, t in (("param", p), ("exp_avg", m), ("exp_avg_sq", v), ("master", master)):
+            codes = eight and what.startswith("exp_avg")
+            if t is not None and (t.shape != shape or not (codes or t.is_floating_point())):
+                raise ValueError(f"{what}/{n} must be {tuple(shape)}, in a float type or both moments in uint8: got "
+                                 f"{t.dtype} {tuple(t.shape)}")
+        blocks = (-(-shape.numel() // K.MOMENT_BLOCK), 2)
+        if eight and (sc.dtype != torch.uint8 or tuple(sc.shape) != blocks):
+            raise ValueError(f"scales/{n} must be uint8 {blocks}, got {sc.dtype} {tuple(sc.shape)}")
+        return p, m, v, sc if eight else None, master
+
     @torch.no_grad()
     def load_state_tensors(self, tensors: dict[str, torch.Tensor], step_count: int) -> None:
         """Copies a state in.  Float moments load into 8 bits as the nearest codes, 8-bit ones into float32
-        as their values; without masters, masters start from the parameters."""
-        for n, p in self.params.items():
-            p.data.copy_(tensors[f"param/{n}"])
-            m, v, sc = (tensors.get(f"{key}/{n}") for key in ("exp_avg", "exp_avg_sq", "scales"))
-            if m is None or v is None or (m.dtype == torch.uint8 and sc is None):
-                raise KeyError(f"the moments of {n} are not all there")
-            mine = self.state[n]
-            if (m.dtype == torch.uint8) != (self.state_bits == 8):
+        as their values; without masters, masters start from the parameters.  A state that lacks something or
+        does not fit is refused before anything is written."""
+        fitting = {n: self._fitting(tensors, n) for n in self.params}
+        for n, (value, m, v, sc, master) in fitting.items():
+            p, mine = self.params[n], self.state[n]
+            p.data.copy_(value)
+            if (sc is not None) != (self.state_bits == 8):
                 m, v = (t.to(p.device) for t in (m, v))
                 if self.state_bits == 8:
                     K.moments_encode(m.float().contiguous(), v.float().contiguous(), mine["exp_avg"],
                                      mine["exp_avg_sq"], mine["scales"])
                 else:
                     m, v = K.moments_decode(m.contiguous(), v.contiguous(), sc.to(p.device).contiguous())
-            if self.state_bits == 32 or m.dtype == torch.uint8:
+            if self.state_bits == 32 or sc is not None:
                 mine["exp_avg"].copy_(m)
                 mine["exp_avg_sq"].copy_(v)
                 if self.state_bits == 8:
                     mine["scales"].copy_(sc)
             if "master" in mine:
-                mine["master"].copy_(tensors.get(f"master/{n}", p.data))
+                mine["master"].copy_(p.data if master is None else master)
         self.step_count = step_count
 
 

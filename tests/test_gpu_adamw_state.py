@@ -175,3 +175,55 @@ def test_negative_and_negative_zero_second_moments():
     bad = np.zeros(n, bool)
     bad[128:256] = bad[384:512] = True
     assert np.array_equal(np.isnan(got), bad)
+
+
+def _state(bits):
+    opt = moe.AdamW({"a": _param(300, 1, torch.bfloat16), "b": _param(20, 2, torch.bfloat16)}, **HYPER, state_bits=bits,
+                    master_weights=True)
+    for p in opt.params.values():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    return opt
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("change", [
+    lambda t: t.pop("param/b"),
+    lambda t: t.pop("exp_avg_sq/b"),
+    lambda t: t.update({"exp_avg/b": t["exp_avg/b"].to(torch.uint8 if t["exp_avg/b"].is_floating_point() else torch.float32)}),
+    lambda t: t.update({"exp_avg/b": t["exp_avg/b"][:1]}),
+    lambda t: t.update({"exp_avg_sq/b": t["exp_avg_sq/b"].view(2, 10)}),
+    lambda t: t.update({"param/b": t["param/b"][:1]}),
+    lambda t: t.update({"master/b": t["master/b"][:1]}),
+    lambda t: t.update({"param/b": t["param/b"].to(torch.uint8)}),
+    lambda t: t.update({"master/b": t["master/b"].to(torch.int32)}),
+    lambda t: t.update({"exp_avg/b": t["exp_avg/b"].to(torch.int32), "exp_avg_sq/b": t["exp_avg_sq/b"].to(torch.int32)}),
+], ids=["no-param", "no-moment", "mixed-widths", "short-moment", "reshaped-moment", "short-param", "short-master",
+        "int-param", "int-master", "int-moments"])
+def test_a_state_that_does_not_fit_changes_nothing(bits, change):
+    saved = {k: t.clone() for k, t in _state(bits).state_tensors().items()}
+    opt = _state(bits)
+    opt.step()
+    before = {k: t.clone() for k, t in opt.state_tensors().items()}
+    change(saved)
+    say(f"adamw state that does not fit {bits}")
+    with pytest.raises((KeyError, ValueError)):
+        opt.load_state_tensors(saved, 1)
+    assert opt.step_count == 2
+    for k, t in opt.state_tensors().items():
+        assert torch.equal(t, before[k]), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_scales_that_do_not_fit_change_nothing(bits):
+    """Of one row (which a copy would spread over all blocks), or of another type."""
+    saved = {k: t.clone() for k, t in _state(8).state_tensors().items()}
+    opt = _state(bits)
+    before = {k: t.clone() for k, t in opt.state_tensors().items()}
+    for sc in (saved["scales/a"][:1], saved["scales/a"].float(), saved["scales/a"].view(-1)):
+        with pytest.raises(ValueError):
+            opt.load_state_tensors({**saved, "scales/a": sc}, 1)
+        for k, t in opt.state_tensors().items():
+            assert torch.equal(t, before[k]), k
+    opt.load_state_tensors(saved, 7)
+    assert opt.step_count == 7 and torch.equal(opt.params["a"].detach(), saved["param/a"])
