@@ -165,13 +165,16 @@ int rhp_route_bwd(const void* dgates, const void* gates, const void* logits, con
  *   dx[t] = dout[t] + sum_j dxp[pair_row[t*k+j]] + sum_j dlogits_sel[t,j] * router_w[topi[t,j]]
  *           + sum_s shared_dx[s][t]
  * (residual + scatter-add of the permuted input gradient + router input gradient).
- * dout may be NULL: no residual term (the layer behind a norm, whose residual
- * passes the norm by).
  * dout, dxp, dx, shared_dx: dtype; dlogits_sel, router_w: r_dtype.
  */
 int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
                   const int32_t* topi, const void* router_w, int r_dtype, const void* const* shared_dx, int n_shared,
                   int dtype, int64_t T, int h, int E, int k, void* dx, hipStream_t stream);
+
+/* The same without dout's term: the layer behind a norm, whose residual passes the norm by. */
+int rhp_token_bwd_no_residual(const void* dxp, const int32_t* pair_row, const void* dlogits_sel, const int32_t* topi,
+                              const void* router_w, int r_dtype, const void* const* shared_dx, int n_shared, int dtype,
+                              int64_t T, int h, int E, int k, void* dx, hipStream_t stream);
 
 /* Workspace bytes rhp_router_wgrad needs. */
 size_t rhp_router_wgrad_workspace_bytes(int64_t T, int h, int E, int k, int r_dtype);

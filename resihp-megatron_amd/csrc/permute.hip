@@ -1066,10 +1066,10 @@ extern "C" int rhp_combine_bwd_fp8(const void* dout, const void* y, const float*
     return check_launch("combine_bwd_bf16_kernel");
 }
 
-extern "C" int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
-                             const int32_t* topi, const void* router_w, int r_dtype, const void* const* shared_dx,
-                             int n_shared, int dtype, int64_t T, int h, int E, int k, void* dx, hipStream_t stream) {
-    clear_error();
+// dout null: without the residual's term.
+static int token_bwd(const void* dout, const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
+                     const int32_t* topi, const void* router_w, int r_dtype, const void* const* shared_dx,
+                     int n_shared, int dtype, int64_t T, int h, int E, int k, void* dx, hipStream_t stream) {
     if (int rc = check_rows("rhp_token_bwd", dtype, T, h, k)) return rc;
     RHP_REQUIRE(E >= 1 && n_shared >= 0 && n_shared <= kMaxShared, "rhp_token_bwd: bad E or n_shared");
     if (T == 0) return 0;
@@ -1141,6 +1141,24 @@ extern "C" int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* p
                                n_shared, T, h, E, k, static_cast<float*>(dx));
     }
     return check_launch("token_bwd_kernel");
+}
+
+extern "C" int rhp_token_bwd(const void* dout, const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
+                             const int32_t* topi, const void* router_w, int r_dtype, const void* const* shared_dx,
+                             int n_shared, int dtype, int64_t T, int h, int E, int k, void* dx, hipStream_t stream) {
+    clear_error();
+    RHP_REQUIRE(dout || T <= 0, "rhp_token_bwd: null or unaligned pointer");
+    return token_bwd(dout, dxp, pair_row, dlogits_sel, topi, router_w, r_dtype, shared_dx, n_shared, dtype, T, h, E, k,
+                     dx, stream);
+}
+
+extern "C" int rhp_token_bwd_no_residual(const void* dxp, const int32_t* pair_row, const void* dlogits_sel,
+                                         const int32_t* topi, const void* router_w, int r_dtype,
+                                         const void* const* shared_dx, int n_shared, int dtype, int64_t T, int h, int E,
+                                         int k, void* dx, hipStream_t stream) {
+    clear_error();
+    return token_bwd(nullptr, dxp, pair_row, dlogits_sel, topi, router_w, r_dtype, shared_dx, n_shared, dtype, T, h, E,
+                     k, dx, stream);
 }
 
 extern "C" size_t rhp_router_wgrad_workspace_bytes(int64_t T, int h, int E, int k, int r_dtype) {

@@ -307,8 +307,12 @@ def token_bwd(dout: torch.Tensor, dxp: torch.Tensor | None, pair_row: torch.Tens
         _expect(_rows_of(t, f"shared_dx[{i}]", h, dout.dtype) == T, "shared gradients need one row per token")
     dx = torch.empty_like(dout)
     arr = C.ptr_array([s.data_ptr() for s in shared_dx])
-    _call("rhp_token_bwd", dev, _ptr(dout) if residual else None, _ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi),
-          _ptr(router_w), dtype_code(router_w), arr, len(shared_dx), dtype_code(dout), T, h, router_w.shape[0], k, _ptr(dx))
+    args = (_ptr(dxp), _ptr(pair_row), _ptr(dl), _ptr(topi), _ptr(router_w), dtype_code(router_w), arr, len(shared_dx),
+            dtype_code(dout), T, h, router_w.shape[0], k, _ptr(dx))
+    if residual:
+        _call("rhp_token_bwd", dev, _ptr(dout), *args)
+    else:
+        _call("rhp_token_bwd_no_residual", dev, *args)
     return dx
 
 

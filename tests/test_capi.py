@@ -152,3 +152,14 @@ def test_fp8_row_entries_reject_bad_arguments(entry, kw, msg):
 def test_combine_bwd_fp8_rejects_top_k_above_8():
     with pytest.raises(RuntimeError, match="top-k above 8"):
         _row_codes("rhp_combine_bwd_fp8", k=9)
+
+
+@pytest.mark.parametrize("entry", ["rhp_token_bwd", "rhp_token_bwd_no_residual"])
+def test_token_bwd_takes_no_null_gradient(entry):
+    """The residual's gradient is left out by the entry without it, not by a null pointer."""
+    fake = ctypes.c_void_p(4096)   # never dereferenced: validation fails first
+    lead = (None,) if entry == "rhp_token_bwd" else ()
+    dx = fake if lead else None
+    with pytest.raises(RuntimeError, match="null or unaligned pointer"):
+        C.call(entry, *lead, fake, fake, fake, fake, fake, C.F32, C.ptr_array([]), 0, C.BF16, 4, 64, 8, 2, dx, None)
+    C.call(entry, *lead, fake, fake, fake, fake, fake, C.F32, C.ptr_array([]), 0, C.BF16, 0, 64, 8, 2, dx, None)
