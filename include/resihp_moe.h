@@ -513,6 +513,11 @@ int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes,
                    const int* g_dtypes, double lr, double beta1, double beta2, double eps, double weight_decay,
                    int64_t step, const float* grad_scale, uint64_t seed, hipStream_t stream);
 
+/* The same for a plan of F64 weights, with grad_scale in double (rhp_grad_norm64's out + 1), not NULL. */
+int rhp_adamw_step64(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
+                     const int* g_dtypes, double lr, double beta1, double beta2, double eps, double weight_decay,
+                     int64_t step, const double* grad_scale, hipStream_t stream);
+
 /*
  * The values that n codes stand for, as bfloat16 (which holds each exactly),
  * and the codes nearest to n float moments.  scales: [ceil(n/128)][2] bytes.
@@ -529,13 +534,18 @@ size_t rhp_grad_norm_workspace_bytes(int count);
 /*
  * out[0] = the 2-norm of all elements of the gradients, out[1] = min(1,
  * max_norm / (out[0] + 1e-6)), what clips them (rhp_adamw_step's grad_scale).
- * Summed in double: no square overflows, and the order is fixed.  A NaN or an
+ * Summed in double: no square of a float overflows, one of a double past 1e154
+ * does; the order is fixed.  A NaN or an
  * infinity among the gradients makes the norm that, and the coefficient NaN or
  * 0.  Gradients may mix F64/F32/BF16 and need their element's alignment; NULL
  * entries are skipped.
  */
 int rhp_grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel, double max_norm,
                   float* out, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The same with the results in double, as float64 gradients need them (a float's rounding and range are less). */
+int rhp_grad_norm64(int count, const void* const* grads, const int* dtypes, const int64_t* numel, double max_norm,
+                    double* out, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------ fp8 experts (delayed scaling) */
 

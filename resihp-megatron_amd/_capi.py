@@ -66,10 +66,12 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "rhp_adamw_plan_bytes": (_sz, [_i, _p, _i]),
     "rhp_adamw_plan": (_i, [_i, _pp, _p, _pp, _pp, _pp, _pp, _p, _p, _p, _i, _p, _sz]),
     "rhp_adamw_step": (_i, [_p, _p, _sz, _pp, _p, _d, _d, _d, _d, _d, _i64, _p, _u64, _p]),
+    "rhp_adamw_step64": (_i, [_p, _p, _sz, _pp, _p, _d, _d, _d, _d, _d, _i64, _p, _p]),
     "rhp_moments_decode": (_i, [_p, _p, _p, _i64, _p, _p, _p]),
     "rhp_moments_encode": (_i, [_p, _p, _i64, _p, _p, _p, _p]),
     "rhp_grad_norm_workspace_bytes": (_sz, [_i]),
     "rhp_grad_norm": (_i, [_i, _pp, _p, _p, _d, _p, _p, _sz, _p]),
+    "rhp_grad_norm64": (_i, [_i, _pp, _p, _p, _d, _p, _p, _sz, _p]),
     "rhp_fp8_padded_offsets": (_i, [_p, _i, _i, _p, _p]),
     "rhp_fp8_cast": (_i, [_p, _i, _i64, _i, _i, _p, _p, _i64, _p, _i, _i, _i, _p, _p, _p, _p, _p]),
     "rhp_fp8_cast_many": (_i, [_i, _pp, _pi64, _pi64, _pp, _i, _i, _i, _pp, _pp, _pp, _p]),

@@ -366,8 +366,8 @@ constexpr double kLeastFastEps = 2e-12;   // times ibc2s
 __device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return a * b + c; }
 
-template <int N, bool kTinyEps, class A>
-__device__ __forceinline__ void update(const Scalars<A>& s, A keep, const float* grad_scale, A* p, A* g, A* m, A* v) {
+template <int N, bool kTinyEps, class A, class G>
+__device__ __forceinline__ void update(const Scalars<A>& s, A keep, const G* grad_scale, A* p, A* g, A* m, A* v) {
     if (grad_scale) {
         const A gs = static_cast<A>(*grad_scale);
 #pragma unroll
@@ -424,11 +424,12 @@ template <int N, class A> __device__ __forceinline__ void store_weight(const Pla
     }
 }
 
-template <class A, bool kState8, bool kTinyEps>
+// G: the type of *grad_scale, double only for double weights.
+template <class A, bool kState8, bool kTinyEps, class G>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const PlanTensor* __restrict__ tensors,
                                                          const uint32_t* __restrict__ of_block, Grads grads,
                                                          uint32_t t0, uint32_t b0, Scalars<A> s,
-                                                         const float* __restrict__ grad_scale, uint32_t salt) {
+                                                         const G* __restrict__ grad_scale, uint32_t salt) {
     const uint32_t b = b0 + blockIdx.x;
     const uint32_t ti = of_block[b];
     const PlanTensor t = tensors[ti];
@@ -580,8 +581,9 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormTensors ts, dou
 // One block: the launch and 2048 loads, 4 us.  In a launch of its own, so that no counter has to be zero before a
 // call and none is shared between two.  out = [norm, min(1, max_norm / (norm + 1e-6))]; a norm that is NaN makes
 // the coefficient NaN.
+template <class O>
 __global__ __launch_bounds__(kThreads) void grad_norm_finish_kernel(const double* __restrict__ part, int n,
-                                                                    double max_norm, float* __restrict__ out) {
+                                                                    double max_norm, O* __restrict__ out) {
     __shared__ double s[kThreads / 64];
     double sum = 0;
     for (int i = threadIdx.x; i < n; i += kThreads) sum += part[i];
@@ -589,8 +591,8 @@ __global__ __launch_bounds__(kThreads) void grad_norm_finish_kernel(const double
     if (threadIdx.x == 0) {
         const double norm = __builtin_sqrt(sum);
         const double c = max_norm / (norm + 1e-6);
-        out[0] = static_cast<float>(norm);
-        out[1] = static_cast<float>(c >= 1.0 ? 1.0 : c);
+        out[0] = static_cast<O>(norm);
+        out[1] = static_cast<O>(c >= 1.0 ? 1.0 : c);
     }
 }
 
@@ -602,9 +604,9 @@ inline uint64_t tag(const void* p, int dt) {
     return reinterpret_cast<uint64_t>(p) | static_cast<uint64_t>(dt) << kDtypeShift;
 }
 
-template <class A, bool kState8, bool kTinyEps>
+template <class A, bool kState8, bool kTinyEps, class G>
 int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grads, const int* g_dtypes,
-                const Scalars<A>& s, const float* grad_scale, uint32_t salt, hipStream_t stream) {
+                const Scalars<A>& s, const G* grad_scale, uint32_t salt, hipStream_t stream) {
     const PlanHeader& head = *reinterpret_cast<const PlanHeader*>(host);
     const PlanTensor* ts = reinterpret_cast<const PlanTensor*>(host + sizeof(PlanHeader));
     const PlanTensor* tensors = reinterpret_cast<const PlanTensor*>(dev + sizeof(PlanHeader));
@@ -617,8 +619,8 @@ int launch_step(const uint8_t* host, const uint8_t* dev, const void* const* grad
         for (uint32_t t = t0; t < t1; ++t)
             if (grads && grads[t]) g.g[t - t0] = tag(grads[t], g_dtypes[t]);
         for (uint32_t b = b0; b < b1; b += kMaxBlocks) {
-            hipLaunchKernelGGL((adamw_kernel<A, kState8, kTinyEps>), dim3(std::min(b1 - b, kMaxBlocks)), dim3(kThreads),
-                               0, stream, tensors, of_block, g, t0, b, s, grad_scale, salt);
+            hipLaunchKernelGGL((adamw_kernel<A, kState8, kTinyEps, G>), dim3(std::min(b1 - b, kMaxBlocks)),
+                               dim3(kThreads), 0, stream, tensors, of_block, g, t0, b, s, grad_scale, salt);
             if (int rc = check_launch("adamw_kernel")) return rc;
         }
     }
@@ -711,11 +713,11 @@ extern "C" int rhp_adamw_plan(int count, void* const* params, const int* dtypes,
     return 0;
 }
 
-extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
-                              const int* g_dtypes, double lr, double beta1, double beta2, double eps,
-                              double weight_decay, int64_t step, const float* grad_scale, uint64_t seed,
-                              hipStream_t stream) {
-    clear_error();
+// grad_scale64: *grad_scale in double, for float64 weights; one of the two is null.
+static int adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
+                      const int* g_dtypes, double lr, double beta1, double beta2, double eps, double weight_decay,
+                      int64_t step, const float* grad_scale, const double* grad_scale64, uint64_t seed,
+                      hipStream_t stream) {
     RHP_REQUIRE(image && image_bytes >= sizeof(PlanHeader) && (reinterpret_cast<uintptr_t>(image) & 7) == 0,
                 "rhp_adamw_step: null, unaligned or short image");
     const uint8_t* host = static_cast<const uint8_t*>(image);
@@ -726,6 +728,7 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
     RHP_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "rhp_adamw_step: betas must be in [0, 1)");
     RHP_REQUIRE(lr >= 0.0 && eps >= 0.0 && weight_decay >= 0.0,
                 "rhp_adamw_step: lr, eps and weight_decay must not be negative");
+    RHP_REQUIRE(!grad_scale64 || head.f64, "rhp_adamw_step64: the plan's weights are not float64");
     if (head.blocks == 0) return 0;
     RHP_REQUIRE(dev_image && aligned16(dev_image), "rhp_adamw_step: null or unaligned device image");
     RHP_REQUIRE(!grads || g_dtypes, "rhp_adamw_step: gradients without their dtypes");
@@ -744,16 +747,36 @@ extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t i
                                   static_cast<uint32_t>(seed >> 32)) ^
                               static_cast<uint32_t>(seed));
     const uint8_t* dev = static_cast<const uint8_t*>(dev_image);
+    if (grad_scale64)
+        return launch_step<double, false, false, double>(host, dev, grads, g_dtypes, d, grad_scale64, salt, stream);
     const auto go = [&](auto launch, const auto& scalars) {
         return launch(host, dev, grads, g_dtypes, scalars, grad_scale, salt, stream);
     };
-    if (head.f64) return go(launch_step<double, false, false>, d);
+    if (head.f64) return go(launch_step<double, false, false, float>, d);
     const Scalars<float> f{static_cast<float>(d.b1), static_cast<float>(d.c1), static_cast<float>(d.b2),
                            static_cast<float>(d.c2), static_cast<float>(d.ibc2s), static_cast<float>(d.eps),
                            static_cast<float>(d.a), static_cast<float>(d.keep)};
     if (eps < kLeastFastEps * ibc2s)
-        return head.state8 ? go(launch_step<float, true, true>, f) : go(launch_step<float, false, true>, f);
-    return head.state8 ? go(launch_step<float, true, false>, f) : go(launch_step<float, false, false>, f);
+        return head.state8 ? go(launch_step<float, true, true, float>, f) : go(launch_step<float, false, true, float>, f);
+    return head.state8 ? go(launch_step<float, true, false, float>, f) : go(launch_step<float, false, false, float>, f);
+}
+
+extern "C" int rhp_adamw_step(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
+                              const int* g_dtypes, double lr, double beta1, double beta2, double eps,
+                              double weight_decay, int64_t step, const float* grad_scale, uint64_t seed,
+                              hipStream_t stream) {
+    clear_error();
+    return adamw_step(image, dev_image, image_bytes, grads, g_dtypes, lr, beta1, beta2, eps, weight_decay, step,
+                      grad_scale, nullptr, seed, stream);
+}
+
+extern "C" int rhp_adamw_step64(const void* image, const void* dev_image, size_t image_bytes, const void* const* grads,
+                                const int* g_dtypes, double lr, double beta1, double beta2, double eps,
+                                double weight_decay, int64_t step, const double* grad_scale, hipStream_t stream) {
+    clear_error();
+    RHP_REQUIRE(grad_scale, "rhp_adamw_step64: null grad_scale");
+    return adamw_step(image, dev_image, image_bytes, grads, g_dtypes, lr, beta1, beta2, eps, weight_decay, step,
+                      nullptr, grad_scale, 0, stream);
 }
 
 static int check_codes(const char* what, int64_t n, const void* const* ptrs, int count) {
@@ -791,14 +814,13 @@ extern "C" size_t rhp_grad_norm_workspace_bytes(int count) {
     return static_cast<size_t>(std::max(1, (count + kNormMax - 1) / kNormMax)) * kNormBlocks * sizeof(double);
 }
 
-extern "C" int rhp_grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel,
-                             double max_norm, float* out, void* workspace, size_t workspace_bytes,
-                             hipStream_t stream) {
-    clear_error();
+template <class O>
+static int grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel, double max_norm,
+                     O* out, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     RHP_REQUIRE(count >= 0, "rhp_grad_norm: count must be >= 0");
     RHP_REQUIRE(count == 0 || (grads && dtypes && numel), "rhp_grad_norm: null array");
     RHP_REQUIRE(max_norm > 0.0, "rhp_grad_norm: max_norm must be positive");
-    RHP_REQUIRE(out && (reinterpret_cast<uintptr_t>(out) & 3) == 0, "rhp_grad_norm: null or unaligned output");
+    RHP_REQUIRE(out && (reinterpret_cast<uintptr_t>(out) & (sizeof(O) - 1)) == 0, "rhp_grad_norm: null or unaligned output");
     RHP_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= rhp_grad_norm_workspace_bytes(count),
                 "rhp_grad_norm: workspace smaller than rhp_grad_norm_workspace_bytes(), null or unaligned");
     for (int i = 0; i < count; ++i) {
@@ -825,6 +847,20 @@ extern "C" int rhp_grad_norm(int count, const void* const* grads, const int* dty
         if (int rc = check_launch("grad_norm_kernel")) return rc;
         parts += nb;
     }
-    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(kThreads), 0, stream, part, parts, max_norm, out);
+    hipLaunchKernelGGL(grad_norm_finish_kernel<O>, dim3(1), dim3(kThreads), 0, stream, part, parts, max_norm, out);
     return check_launch("grad_norm_finish_kernel");
+}
+
+extern "C" int rhp_grad_norm(int count, const void* const* grads, const int* dtypes, const int64_t* numel,
+                             double max_norm, float* out, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream) {
+    clear_error();
+    return grad_norm(count, grads, dtypes, numel, max_norm, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int rhp_grad_norm64(int count, const void* const* grads, const int* dtypes, const int64_t* numel,
+                               double max_norm, double* out, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+    clear_error();
+    return grad_norm(count, grads, dtypes, numel, max_norm, out, workspace, workspace_bytes, stream);
 }

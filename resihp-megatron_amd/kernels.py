@@ -943,24 +943,29 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
     elements, 2^32 with moments in 8 bits).
 
     ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights), or the plan's
-    ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device that
-    every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the random bits that round
+    ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device (or float64
+    with float64 weights) that every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the random bits that round
     moments of 8 bits.  A graph that captures the step needs the plan for as long as it is replayed."""
     if not isinstance(grads, PlanGrads):
         grads = PlanGrads(plan, grads)
     if grads.plan is not plan:
         raise KernelArgumentError("the gradients are another AdamW plan's")
+    double = grad_scale is not None and grad_scale.dtype == torch.float64
     if grad_scale is not None:
-        _expect(grad_scale.dtype == torch.float32 and grad_scale.numel() == 1 and grad_scale.device == plan.device,
-                "grad_scale must be one float32 on the plan's device")
+        _expect((grad_scale.dtype == torch.float32 or (double and plan.dtypes[0] is torch.float64))
+                and grad_scale.numel() == 1 and grad_scale.device == plan.device,
+                "grad_scale must be one float32 (or float64 with float64 weights) on the plan's device")
     if torch.cuda.is_current_stream_capturing():
         plan.captured = True
     elif torch._C._cuda_getCurrentRawStream(plan.device.index) != plan.stream:
         # Should the plan be dropped while this step runs, its memory waits for this stream too.
         plan.dev_image.record_stream(torch.cuda.current_stream(plan.device))
-    _call("rhp_adamw_step", plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(),
-          grads.ptrs, grads.codes, float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
-          int(step), _ptr(grad_scale), int(seed) & 0xFFFFFFFFFFFFFFFF)
+    args = (plan.device, plan.image.data_ptr(), plan.dev_image.data_ptr(), plan.image.numel(), grads.ptrs, grads.codes,
+            float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step), _ptr(grad_scale))
+    if double:
+        _call("rhp_adamw_step64", *args)
+    else:
+        _call("rhp_adamw_step", *args, int(seed) & 0xFFFFFFFFFFFFFFFF)
 
 
 def _check_moments(q_m, q_v, scales) -> int:
@@ -991,9 +996,9 @@ def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: tor
     _call("rhp_moments_encode", dev, _ptr(m), _ptr(v), n, _ptr(q_m), _ptr(q_v), _ptr(scales))
 
 
-def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
-    """float32 [2] on the device: the 2-norm over all elements of all gradients (summed in float64), and
-    min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
+def grad_norm(grads, max_norm: float = float("inf"), dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """[2] in ``dtype`` (float32 or float64) on the device: the 2-norm over all elements of all gradients (summed
+    in float64), and min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
     one device, None entries skipped; or a plan's ``PlanGrads``."""
     grads = grads if isinstance(grads, PlanGrads) else list(grads)
     if isinstance(grads, PlanGrads):
@@ -1015,10 +1020,11 @@ def grad_norm(grads, max_norm: float = float("inf")) -> torch.Tensor:
         numel = _host_array(ctypes.c_int64, list(map(_T.numel, grads)))
     if not max_norm > 0:
         raise KernelArgumentError(f"max_norm must be positive, got {max_norm}")
-    out = torch.empty(2, dtype=torch.float32, device=dev)
+    _expect(dtype in (torch.float32, torch.float64), f"the norm is float32 or float64, not {dtype}")
+    out = torch.empty(2, dtype=dtype, device=dev)
     ws_bytes = C.lib().rhp_grad_norm_workspace_bytes(n)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call("rhp_grad_norm", dev, n, ptrs, codes, numel, float(max_norm), out.data_ptr(), ws.data_ptr(), ws_bytes)
+    _call("rhp_grad_norm" if dtype is torch.float32 else "rhp_grad_norm64", dev, n, ptrs, codes, numel, float(max_norm), out.data_ptr(), ws.data_ptr(), ws_bytes)
     return out
 
 

@@ -288,7 +288,7 @@ class AdamW:
     rounded: ``seed``, the step and the parameter's name give the random bits, so a run is reproducible and
     a parameter keeps its own when it moves).  ``master_weights``: float32 masters of the bfloat16
     parameters, which are then the masters' rounded values.  ``max_grad_norm``: clips; ``grad_norm`` then
-    holds the last step's [norm, coefficient] on the device.  ``no_decay``: names without weight decay; like
+    holds the last step's [norm, coefficient] on the device (float64 for float64 parameters).  ``no_decay``: names without weight decay; like
     ``lr`` and ``weight_decay``, what it is at a step counts.
 
     The state lives in a few flat buffers (``buffers()``), each tensor from a multiple of 128 elements on,
@@ -372,7 +372,10 @@ class AdamW:
             grads = K.PlanGrads(plan, grads, moved=False)
         except K.KernelArgumentError:   # gradients with strides, or what a copy does not mend
             grads = K.PlanGrads(plan, [None if g is None else g.contiguous() for g in grads], moved=False)
-        norm = K.grad_norm(grads, self.max_grad_norm) if self.max_grad_norm is not None and grads.any else None
+        norm = None
+        if self.max_grad_norm is not None and grads.any:
+            norm = K.grad_norm(grads, self.max_grad_norm,
+                               torch.float64 if plan.dtypes[0] is torch.float64 else torch.float32)
         K.adamw_step(plan, grads, self.lr, self.betas, self.eps, self.weight_decay, self.step_count + 1,
                      None if norm is None else norm[1:], self.seed)
         # The kernel writes the parameters behind torch's back: a graph that still holds them has to notice.

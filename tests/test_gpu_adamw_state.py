@@ -227,3 +227,45 @@ def test_scales_that_do_not_fit_change_nothing(bits):
             assert torch.equal(t, before[k]), k
     opt.load_state_tensors(saved, 7)
     assert opt.step_count == 7 and torch.equal(opt.params["a"].detach(), saved["param/a"])
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e60])
+def test_clipped_step_of_float64_weights(scale):
+    """The coefficient that clips float64 gradients is float64: neither its rounding to float32 nor float32's range
+    comes into the step.  The norm's sum of 5000 squares and the coefficient are off by at most 40 u, m by 4 u more
+    and v by twice that; the update's own 16 u."""
+    n = 5000
+    opt = moe.AdamW({"p": torch.nn.Parameter(seeded((n,), 1, 0.05).double().to(DEV))}, **HYPER, max_grad_norm=0.5)
+    p = opt.params["p"]
+    p.grad = seeded((n,), 2).double().to(DEV) * scale
+    w, g = p.detach().cpu().numpy().copy(), p.grad.cpu().numpy()
+    say(f"adamw f64 clip {scale}")
+    opt.step()
+    norm = float(np.sqrt((g ** 2).sum()))
+    coef = min(1.0, 0.5 / (norm + 1e-6))
+    u = 2.0 ** -53
+    got = opt.grad_norm.tolist()
+    assert opt.grad_norm.dtype == torch.float64
+    assert abs(got[0] - norm) <= 40 * u * norm and abs(got[1] - coef) <= 44 * u * coef
+    m, v = (1 - 0.9) * coef * g, (1 - 0.95) * (coef * g) ** 2
+    assert (np.abs(opt.state["p"]["exp_avg"].cpu().numpy() - m) <= 52 * u * np.abs(m)).all()
+    assert (np.abs(opt.state["p"]["exp_avg_sq"].cpu().numpy() - v) <= 104 * u * v).all()
+    want = R.weight(w, m, v, np.float64, *HYPER.values(), 1)
+    tol = u * (4 * np.abs(w) + 130 * np.abs(want - w * (1 - HYPER["lr"] * HYPER["weight_decay"])))
+    assert (np.abs(p.detach().cpu().numpy() - want) <= tol).all()
+
+
+def test_a_float64_coefficient_is_for_float64_weights():
+    say("adamw float64 coefficient")
+    z = lambda n, dt=torch.float32: torch.zeros(n, dtype=dt, device=DEV)  # noqa: E731
+    one = torch.ones(1, dtype=torch.float64, device=DEV)
+    step = lambda plan, dt, c: K.adamw_step(plan, [z(10, dt)], 1e-3, (0.9, 0.999), 1e-8, 0.0, 1, c)  # noqa: E731
+    plans = {dt: K.AdamWPlan([z(10, dt)], [z(10, dt)], [z(10, dt)]) for dt in (torch.float32, torch.float64)}
+    step(plans[torch.float64], torch.float64, one)
+    step(plans[torch.float64], torch.float64, one.float())
+    with pytest.raises(RuntimeError):
+        step(plans[torch.float32], torch.float32, one)
+    g = [seeded((777,), 1).to(DEV), seeded((5,), 2).to(torch.bfloat16).to(DEV)]
+    assert torch.equal(K.grad_norm(g, 0.5, torch.float64).float(), K.grad_norm(g, 0.5))
+    with pytest.raises(RuntimeError):
+        K.grad_norm(g, 0.5, torch.bfloat16)
