@@ -109,3 +109,59 @@ def test_column_sums_of_very_many_rows(T, h):
     want_w = (dy[0].double() * 0.5 * rstd[0].double()) * T
     _close(db, want_b, tol * want_b.abs(), "db")
     _close(dw, want_w, tol * want_w.abs(), "dw")
+
+
+def _rows(dt, h, res):
+    """Rows that the register kernels' 256 blocks hold at a time in the backward: each of its groups has one.  (How
+    many threads have a row is the kernels' choice; what counts here is that groups walk several rows.)"""
+    chunks = -(-h * torch.finfo(dt).bits // 128)
+    for tpr, nv in ((8, 2), (16, 2), (32, 2), (64, 2), (64, 3), (64, 4), (128, 2), (192, 2), (256, 2), (384, 2), (512, 2)):
+        if chunks <= tpr * nv and (nv < 4 or not res and h * torch.finfo(dt).bits % 128 == 0):
+            threads = 576 if tpr == 192 else 512 if tpr < 384 else 768 if tpr == 384 else tpr
+            return 256 * (threads // tpr)
+    return 256
+
+
+# Rows on 8, 16 and 32 lanes, on a wave with two, three and four chunks, on 128 to 1024 threads; whole and cut chunks.
+@pytest.mark.parametrize("dt,h", [(torch.bfloat16, h) for h in (64, 100, 250, 500, 1000, 1100, 1536, 1800, 2048, 2500,
+                                                                2816, 4000, 4099, 6000, 6144, 8000, 12001, 16384)] +
+                         [(torch.float32, h) for h in (60, 250, 700, 768, 1000, 1400, 3000, 4000, 8192)])
+@pytest.mark.parametrize("res", [False, True])
+def test_groups_that_walk_several_rows(dt, h, res):
+    """Two or three rows a group, against float64: the row after the first has its loads ahead, or none, and its terms
+    in the same column sums.  A column's sum: three additions in a lane, three between a wave's groups, four
+    between a block's parts, 16 + 15 over the partial rows, the term's own three roundings and the result's."""
+    T = 2 * _rows(dt, h, res) + 37
+    say(f"norm several rows T={T} h={h} {dt} res={res}")
+    g = torch.Generator(device=DEV).manual_seed(h)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    x, dy = (rand(T, h) * 2 + 0.3).to(dt), rand(T, h).to(dt)
+    w, b, dres = 1 + 0.1 * rand(h), 0.1 * rand(h), rand(T, h).to(dt) if res else None
+    y, mean, rstd = K.layer_norm(x, w, b, 1e-5)
+    dx, dw, db = K.layer_norm_bwd(dy, x, w, mean, rstd, dres=dres)
+    half, D = torch.finfo(dt).eps / 2, 32 + 10 + 16     # additions: in a lane, over its lanes, over the waves
+    xd, dyd, wd = x.double(), dy.double(), w.double()
+    m = xd.mean(1, keepdim=True)
+    c = xd - m
+    var = (c * c).mean(1, keepdim=True)
+    r = (var + 1e-5).rsqrt()
+    em = (D + 2) * U * xd.abs().mean(1, keepdim=True)
+    ev = (D + 4) * U * var + em * em + 2 * U * (c.abs() * xd.abs()).mean(1, keepdim=True)
+    er = r * (0.5 * ev / (var + 1e-5) + 4 * U)
+    _close(mean, m[:, 0], em[:, 0], "mean")
+    _close(rstd, r[:, 0], er[:, 0], "rstd")
+    want = c * r * wd + b.double()
+    tol = wd.abs() * (r * (em + U * c.abs()) + c.abs() * er + 2 * U * c.abs() * r) + 2 * U * (want.abs() + b.double().abs())
+    _close(y, want, tol * 1.01 + (want.abs() + tol) * half, "y")
+    m, r = mean.double()[:, None], rstd.double()[:, None]
+    gd, xh = dyd * wd, (xd - m) * r
+    c1, c2 = (gd * xh).mean(1, keepdim=True), gd.mean(1, keepdim=True)
+    a1, a2 = (gd * xh).abs().mean(1, keepdim=True), gd.abs().mean(1, keepdim=True)
+    want = r * (gd - c2 - xh * c1)
+    tol = r * U * (3 * gd.abs() + (D + 4) * a2 + xh.abs() * ((D + 8) * a1 + 6 * c1.abs()) + 4 * c2.abs())
+    if res:
+        want = want + dres.double()
+        tol = tol + U * want.abs()
+    _close(dx, want, tol * 1.01 + (want.abs() + tol) * half, "dx")
+    for got, terms, name in ((dw, dyd * xh, "dw"), (db, dyd, "db")):
+        _close(got, terms.sum(0), (3 + 3 + 4 + 16 + 15 + 4) * U * terms.abs().sum(0), name)
