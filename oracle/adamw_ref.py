@@ -41,6 +41,7 @@ def weight(p, m, v, dtype, lr, betas, eps, weight_decay, step, decay=True):
 
 
 def mix(x):
+    """A 32-bit hash: lowbias32 as C. Wellons published it (hash prospector)."""
     x = np.asarray(x, np.uint64) & np.uint64(M32)
     x = ((x ^ (x >> np.uint64(16))) * np.uint64(0x7FEB352D)) & np.uint64(M32)
     x = ((x ^ (x >> np.uint64(15))) * np.uint64(0x846CA68B)) & np.uint64(M32)

@@ -107,7 +107,8 @@ template <int N, class W> __device__ __forceinline__ void load_again(const W* p,
 // One block a row, any h: the row is read again for every pass, from the
 // caches.  For float64, and for rows that are too short or too long for
 // registers (below).  3355 rows of 20000 bfloat16: forward 78 us, 3.5 TB/s;
-// backward 164 us, which reads dy and x a second time for the columns' sums.
+// backward with the residual's gradient 186 us, which reads dy and x a second
+// time for the columns' sums.  float64, 16384 rows of 4096: 298 and 644 us.
 //
 // A thread's share of a row has no bound but h / 256, so the sums B of rows
 // past the registers are double: the values of a chunk are added in pairs in
@@ -357,8 +358,9 @@ __global__ __launch_bounds__(kReduceThreads) void norm_bwd_reduce_kernel(const A
 //
 // The shape is the smallest that holds the row, since idle lanes cost: 64 M
 // bfloat16 in rows of 64 took 364 us on a wave a row, 54 on 8 lanes; in rows
-// of 2560 52 us forward and 110 backward on 256 threads, 48 and 94 on 192; in
-// rows of 1100 68 and 137 on 128 threads, 49 and 103 on 64 with three chunks.
+// of 2560 52 us forward and 117 backward on 256 threads, 48 and 105 on 192; in
+// rows of 1100 69 and 139 on 128 threads, 49 and 98 to 106 on 64 with three
+// chunks.
 // A row within a wave also spares the barriers, which shows where the backward
 // has no residual to read: rows of 2048 76 us on 128 threads, 65 on 64 with
 // four chunks.  With a residual both take 94, and of few rows the four chunks
@@ -521,7 +523,7 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     W* __restrict__ dw, W* __restrict__ db, float* __restrict__ part) {
     constexpr int N = kVec<S>, G = bwd_threads(TPR) / TPR;
     // 16 waves a block, or four chunks a thread, leave no registers for the next row (16 waves of bfloat16 spill a
-    // few all the same: rows of 12288 and 16384 run at 5.9 TB/s).
+    // few all the same: rows of 12288 and 16384 run at 5.0 to 5.5 TB/s).
     constexpr bool kAhead = TPR < 1024 && NV < 4;
     __shared__ float red[2][bwd_threads(TPR) / 64][2];
     const int grp = group_of<TPR>();
@@ -602,7 +604,8 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     }
     if (!dw && !db) return;
     // The block's rows: the sums of a wave's groups, then the waves' (or groups') one after the other, then a
-    // partial row each of dw and db (or the result itself, if this block had all rows).
+    // partial row each of dw and db (or the result itself, if this block had all rows).  All of it is float: 1500 rows of
+// 1365 float32 are off by 1.2e-7 of themselves (rms), where a sum in double, rounded once, is off by 0.4e-7.
     if constexpr (TPR < 64) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
