@@ -604,8 +604,8 @@ __global__ __launch_bounds__(bwd_threads(TPR)) void norm_bwd_reg_kernel(
     }
     if (!dw && !db) return;
     // The block's rows: the sums of a wave's groups, then the waves' (or groups') one after the other, then a
-    // partial row each of dw and db (or the result itself, if this block had all rows).  All of it is float: 1500 rows of
-// 1365 float32 are off by 1.2e-7 of themselves (rms), where a sum in double, rounded once, is off by 0.4e-7.
+    // partial row each of dw and db (or the result itself, if this block had all rows).  All of it is float: 1500
+    // rows of 1365 float32 are off by 1.2e-7 of themselves (rms), where a sum in double, rounded once, is off by 0.4e-7.
     if constexpr (TPR < 64) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)

@@ -944,8 +944,9 @@ def adamw_step(plan: AdamWPlan, grads, lr: float, betas: tuple[float, float], ep
 
     ``grads``: float32 or bfloat16 whatever the weight's type (float64 for float64 weights), or the plan's
     ``PlanGrads``; None steps with zeros.  ``grad_scale``: float32 tensor of one element on the device (or float64
-    with float64 weights) that every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the random bits that round
-    moments of 8 bits.  A graph that captures the step needs the plan for as long as it is replayed."""
+    with float64 weights) that every gradient is multiplied with.  ``step`` counts from 1.  ``seed``: of the
+    random bits that round moments of 8 bits.  A graph that captures the step needs the plan for as long as it
+    is replayed."""
     if not isinstance(grads, PlanGrads):
         grads = PlanGrads(plan, grads)
     if grads.plan is not plan:
@@ -998,8 +999,8 @@ def moments_encode(m: torch.Tensor, v: torch.Tensor, q_m: torch.Tensor, q_v: tor
 
 def grad_norm(grads, max_norm: float = float("inf"), dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """[2] in ``dtype`` (float32 or float64) on the device: the 2-norm over all elements of all gradients (summed
-    in float64), and min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three dtypes on
-    one device, None entries skipped; or a plan's ``PlanGrads``."""
+    in float64), and min(1, max_norm / (norm + 1e-6)), which clips them.  ``grads``: tensors of any of the three
+    dtypes on one device, None entries skipped; or a plan's ``PlanGrads``."""
     grads = grads if isinstance(grads, PlanGrads) else list(grads)
     if isinstance(grads, PlanGrads):
         dev, n, ptrs, codes, numel = grads.plan.device, len(grads.grads), grads.ptrs, grads.codes, grads.plan.numel
@@ -1024,7 +1025,8 @@ def grad_norm(grads, max_norm: float = float("inf"), dtype: torch.dtype = torch.
     out = torch.empty(2, dtype=dtype, device=dev)
     ws_bytes = C.lib().rhp_grad_norm_workspace_bytes(n)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call("rhp_grad_norm" if dtype is torch.float32 else "rhp_grad_norm64", dev, n, ptrs, codes, numel, float(max_norm), out.data_ptr(), ws.data_ptr(), ws_bytes)
+    _call("rhp_grad_norm" if dtype is torch.float32 else "rhp_grad_norm64", dev, n, ptrs, codes, numel,
+          float(max_norm), out.data_ptr(), ws.data_ptr(), ws_bytes)
     return out
 
 

@@ -288,8 +288,8 @@ class AdamW:
     rounded: ``seed``, the step and the parameter's name give the random bits, so a run is reproducible and
     a parameter keeps its own when it moves).  ``master_weights``: float32 masters of the bfloat16
     parameters, which are then the masters' rounded values.  ``max_grad_norm``: clips; ``grad_norm`` then
-    holds the last step's [norm, coefficient] on the device (float64 for float64 parameters).  ``no_decay``: names without weight decay; like
-    ``lr`` and ``weight_decay``, what it is at a step counts.
+    holds the last step's [norm, coefficient] on the device (float64 for float64 parameters).  ``no_decay``:
+    names without weight decay; like ``lr`` and ``weight_decay``, what it is at a step counts.
 
     The state lives in a few flat buffers (``buffers()``), each tensor from a multiple of 128 elements on,
     in the order of ``params``; ``state_tensors()`` names views of it.
@@ -364,9 +364,10 @@ class AdamW:
         plan = self._plan
         if (plan is None or set(self.no_decay) != self._plan_no_decay
                 or not plan.holds(self.params.values()) or plan.moved()):
+            made = self._make_plan()
             if plan is not None and plan.captured:
                 self._captured.append(plan)   # a graph reads its image at every replay
-            plan = self._plan = self._make_plan()
+            plan = self._plan = made
             self._plan_no_decay = set(self.no_decay)
         try:
             grads = K.PlanGrads(plan, grads, moved=False)
