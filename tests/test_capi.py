@@ -163,3 +163,25 @@ def test_token_bwd_takes_no_null_gradient(entry):
     with pytest.raises(RuntimeError, match="null or unaligned pointer"):
         C.call(entry, *lead, fake, fake, fake, fake, fake, C.F32, C.ptr_array([]), 0, C.BF16, 4, 64, 8, 2, dx, None)
     C.call(entry, *lead, fake, fake, fake, fake, fake, C.F32, C.ptr_array([]), 0, C.BF16, 0, 64, 8, 2, dx, None)
+
+
+def test_adamw_step64_is_for_float64_plans():
+    L, fake = C.lib(), ctypes.c_void_p(4096)   # fake: never dereferenced, validation fails first
+    numel, dtypes = (ctypes.c_int64 * 1)(10), (ctypes.c_int * 1)(C.F32)
+    size = L.rhp_adamw_plan_bytes(1, numel, 32)
+    image = (ctypes.c_uint64 * (-(-size // 8)))()
+    C.call("rhp_adamw_plan", 1, C.ptr_array([4096]), dtypes, None, C.ptr_array([8192]), C.ptr_array([16384]), None,
+           numel, None, None, 32, image, size)
+    hyper = (1e-3, 0.9, 0.999, 1e-8, 0.0, 1)
+    with pytest.raises(RuntimeError, match="not float64"):
+        C.call("rhp_adamw_step64", image, fake, size, None, None, *hyper, fake, None)
+    with pytest.raises(RuntimeError, match="null grad_scale"):
+        C.call("rhp_adamw_step64", image, fake, size, None, None, *hyper, None, None)
+
+
+def test_grad_norm64_rejects_bad_arguments():
+    fake, ws = ctypes.c_void_p(4096), C.lib().rhp_grad_norm_workspace_bytes(1)
+    grads, numel, dtypes = C.ptr_array([4096]), (ctypes.c_int64 * 1)(10), (ctypes.c_int * 1)(C.F64)
+    for out, top, space, msg in ((4100, 1.0, ws, "output"), (4096, 0.0, ws, "max_norm"), (4096, 1.0, ws - 1, "workspace")):
+        with pytest.raises(RuntimeError, match=msg):
+            C.call("rhp_grad_norm64", 1, grads, dtypes, numel, top, ctypes.c_void_p(out), fake, space, None)
