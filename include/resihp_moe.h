@@ -743,6 +743,8 @@ int64_t rhp_mx4_padded_rows(int64_t rows, int G);
  * With `offsets` ([G+1] on the device, n == 1) the rows come in groups and, along
  * the columns, group g's rows are placed from
  * sum of roundup(earlier counts, 128) on: C = rhp_mx4_padded_rows(rows, G).
+ * Rows of no group (ahead of offsets[0], from offsets[G] on) are quantised along
+ * their rows and have no place along the columns.
  */
 int rhp_mx4_quantize(int n, const void* const* x, int dtype, int64_t rows, int cols, const int32_t* offsets, int G,
                      void* row_codes, void* row_scales, void* col_codes, void* col_scales, hipStream_t stream);

@@ -372,7 +372,8 @@ extern "C" int rhp_mx4_quantize(int n, const void* const* x, int dtype, int64_t 
     RHP_REQUIRE((!row_codes || row_scales) && (!col_codes || col_scales), "rhp_mx4_quantize: codes without scales");
     RHP_REQUIRE(aligned16(row_codes) && aligned16(row_scales) && aligned16(col_codes) && aligned16(col_scales),
                 "rhp_mx4_quantize: codes and scales must be 16-byte aligned");
-    const int64_t tiles = offsets ? (rows + 127 * (static_cast<int64_t>(G) + 1)) / 128 : (rows + 127) / 128;
+    // With groups a last tile each of the G, of the rows behind them and of those ahead.
+    const int64_t tiles = offsets ? (rows + 127 * (static_cast<int64_t>(G) + 2)) / 128 : (rows + 127) / 128;
     const int64_t ct = (static_cast<int64_t>(cols) + 127) / 128;
     const size_t bytes = dtype_bytes(dtype);
     RHP_REQUIRE(ct * tiles * std::min(n, kMx4Many) < (int64_t(1) << 24), "rhp_mx4_quantize: too many tiles");
