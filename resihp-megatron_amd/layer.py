@@ -65,7 +65,7 @@ class LossTokens(NamedTuple):
 
 
 class RouterLosses(NamedTuple):
-    """Balance loss, z loss and the counts [S, E] they are made of."""
+    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads: they are not written before."""
 
     balance: torch.Tensor
     z: torch.Tensor
@@ -349,14 +349,13 @@ class _MoELayerFn(torch.autograd.Function):
         ctx.meta = meta
         ctx.fp8 = (fp8, q8)
         codes, ctx.mx4 = _mx4_tensors(*q4)
-        # (Not the losses themselves: they are outputs, which hold this context.)
-        ctx.loss = None if loss is None else (loss.counts, loss.tokens)
         if loss is not None:
             ctx.set_materialize_grads(False)   # a loss that nothing came back for costs nothing
         ctx.norm_dtype = None if norm_b is None else norm_b.dtype
         ctx.dims = (T, h, P, G, S)
         ctx.save_for_backward(x, router_w, logits, topi, gates, plan.perm, plan.offsets, plan.pair_row, xp, hpre,
-                              act, y, *(losses or LossTokens()), *codes, *weights,
+                              act, y, *(losses or LossTokens()),
+                              *((None, None) if loss is None else (loss.counts, loss.tokens)), *codes, *weights,
                               *(() if mean is None else (res, norm_w, mean, rstd)))
         ctx.shared = (shared_off, shared_h, shared_a)
         return outs
@@ -366,8 +365,9 @@ class _MoELayerFn(torch.autograd.Function):
         meta = ctx.meta
         T, h, P, G, S = ctx.dims
         (x, router_w, logits, topi, gates, perm, offsets, pair_row, xp, hpre, act, y, *ws) = ctx.saved_tensors
-        n4 = 2 + 2 * sum(r is not None for r in ctx.mx4)
-        over, codes, ws = ws[:2], ws[2:n4], ws[n4:]   # the LossTokens, 4-bit matrices
+        n4 = 4 + 2 * sum(r is not None for r in ctx.mx4)
+        # The LossTokens, what the losses' backward needs, 4-bit matrices.
+        over, (counts, tokens), codes, ws = ws[:2], ws[2:4], ws[4:n4], ws[n4:]
         normed = len(ws) > 2 * (G + S)
         if normed:
             *ws, res, norm_w, mean, rstd = ws
@@ -405,7 +405,6 @@ class _MoELayerFn(torch.autograd.Function):
         # router's gradient.
         loss_dx, loss_dwr = [], None
         if d_balance is not None or d_z is not None:
-            counts, tokens = ctx.loss
             dense = K.router_loss_bwd(d_balance, d_z, logits, topi, counts, tokens, meta.score, *over)
             rdx, loss_dwr = K.router_logits_bwd(dense, x, router_w, need_x, ctx.needs_input_grad[3])
             loss_dx = [rdx] if need_x else []
