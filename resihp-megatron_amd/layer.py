@@ -65,7 +65,7 @@ class LossTokens(NamedTuple):
 
 
 class RouterLosses(NamedTuple):
-    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads: they are not written before."""
+    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads (not to be written before it)."""
 
     balance: torch.Tensor
     z: torch.Tensor
@@ -588,10 +588,11 @@ class Mx4Experts:
         return self.fc1.shape[0]
 
 
-@torch.no_grad()
 def mx4_experts(x: torch.Tensor, offsets: torch.Tensor, experts: Mx4Experts) -> torch.Tensor:
     """fc2(act(fc1(x[r]))) of expert g for the bfloat16 rows r in [offsets[g], offsets[g + 1]), from weights in 4
-    bits.  Without autograd.  Rows of no expert are not computed."""
+    bits.  Without autograd: rows that need a gradient are refused.  Rows of no expert are not computed."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("mx4_experts serves without autograd: call it under torch.no_grad() or on x.detach()")
     act = K.mx4_rows_gemm(x, experts.fc1, offsets, experts.act)
     return K.mx4_rows_gemm(act, experts.fc2, offsets)
 

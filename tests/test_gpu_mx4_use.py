@@ -279,3 +279,17 @@ def test_layer_refuses_other_values_of_mx4(bits):
     cfg = moe.MoEConfig(hidden=32, ffn=32, num_experts=2, top_k=1, dtype=BF16)
     with pytest.raises(ValueError, match="mx4 must be True or an Mx4Experts"):
         L.moe_layer(moe._layer_meta(cfg), rand(4, 32), rand(2, 32, dtype=torch.float32), None, [], [], mx4=bits)
+
+
+def test_served_experts_refuse_rows_that_need_a_gradient():
+    """There is no backward through weights in 4 bits that are only served: the call says so instead of cutting the graph."""
+    experts = L.Mx4Experts(list(rand(2, 32, 64, seed=3)), list(rand(2, 64, 16, seed=4)))
+    x, off = rand(20, 64, seed=5), offsets_of([7, 13])
+    want = L.mx4_experts(x, off, experts)
+    leaf = x.clone().requires_grad_(True)
+    for rows in (leaf, leaf * 1):
+        with pytest.raises(ValueError, match="without autograd"):
+            L.mx4_experts(rows, off, experts)
+        with torch.no_grad():
+            assert torch.equal(L.mx4_experts(rows, off, experts), want)
+        assert torch.equal(L.mx4_experts(rows.detach(), off, experts), want)
