@@ -589,6 +589,7 @@ class EPRuntime:
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         cfg, E = self.cfg, self.cfg.num_experts
+        self.router_losses = None   # they hold the last forward's graph
         if self.comms is not None and self.comms.group(f"ep/{self.gidx}") is not None:
             raise NotImplementedError("cross-GPU expert dispatch is not part of this build; "
                                       "the EP group must be a single device")

@@ -106,6 +106,30 @@ def test_ep_runtime_refuses_cross_gpu_groups():
     assert rt.token_range() == (0, 48)
 
 
+def test_ep_runtime_holds_the_losses_of_one_forward_only(monkeypatch):
+    """The last forward's losses hold its graph: they are gone when the next one starts, also if that one fails."""
+    p = placement.single_device(4, "gpu0")
+    weights = {"router.weight": torch.zeros(4, 8)}
+    weights |= {f"experts.{e}.fc{i}.weight": torch.zeros(8, 8) for e in range(4) for i in (1, 2)}
+    rt = moe.EPRuntime(moe.MoEConfig(num_experts=4, device="cpu", z_coef=0.1), p, "gpu0", ["gpu0"], None, None, weights)
+    held, results = [], [("one",), ("two",), RuntimeError("three")]
+
+    def layer(*a, **kw):
+        held.append(rt.router_losses)
+        r = results[len(held) - 1]
+        if isinstance(r, Exception):
+            raise r
+        return torch.zeros(2, 8), torch.zeros(5), *r
+
+    monkeypatch.setattr(moe, "moe_layer", layer)
+    for want in ("one", "two"):
+        rt.forward(torch.zeros(2, 8))
+        assert rt.router_losses == want
+    with pytest.raises(RuntimeError, match="three"):
+        rt.forward(torch.zeros(2, 8))
+    assert held == [None, None, None] and rt.router_losses is None
+
+
 def test_adam_refuses_host_parameters():
     """The fused optimizer step runs on the GPU only: no silent CPU fallback."""
     opt = moe.Adam({"w": torch.nn.Parameter(torch.zeros(4))})
