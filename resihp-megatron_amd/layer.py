@@ -65,7 +65,7 @@ class LossTokens(NamedTuple):
 
 
 class RouterLosses(NamedTuple):
-    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads (not to be written before it)."""
+    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads (not to be written before)."""
 
     balance: torch.Tensor
     z: torch.Tensor
@@ -355,9 +355,9 @@ class _MoELayerFn(torch.autograd.Function):
         ctx.dims = (T, h, P, G, S)
         ctx.save_for_backward(x, router_w, logits, topi, gates, plan.perm, plan.offsets, plan.pair_row, xp, hpre,
                               act, y, *(losses or LossTokens()),
-                              *((None, None) if loss is None else (loss.counts, loss.tokens)), *codes, *weights,
+                              *((None, None) if loss is None else (loss.counts, loss.tokens)), *codes,
+                              *((shared_off, *shared_h, *shared_a) if S else ()), *weights,
                               *(() if mean is None else (res, norm_w, mean, rstd)))
-        ctx.shared = (shared_off, shared_h, shared_a)
         return outs
 
     @staticmethod
@@ -366,14 +366,16 @@ class _MoELayerFn(torch.autograd.Function):
         T, h, P, G, S = ctx.dims
         (x, router_w, logits, topi, gates, perm, offsets, pair_row, xp, hpre, act, y, *ws) = ctx.saved_tensors
         n4 = 4 + 2 * sum(r is not None for r in ctx.mx4)
-        # The LossTokens, what the losses' backward needs, 4-bit matrices.
+        # The LossTokens, what the losses' backward needs, 4-bit matrices, the shared experts' offsets and rows.
         over, (counts, tokens), codes, ws = ws[:2], ws[2:4], ws[4:n4], ws[n4:]
+        shared_off = shared_h = shared_a = None
+        if S:
+            shared_off, shared_h, shared_a, ws = ws[0], ws[1:1 + S], ws[1 + S:1 + 2 * S], ws[1 + 2 * S:]
         normed = len(ws) > 2 * (G + S)
         if normed:
             *ws, res, norm_w, mean, rstd = ws
         fc1s, fc2s = ws[:G], ws[G:2 * G]
         sfc1s, sfc2s = ws[2 * G:2 * G + S], ws[2 * G + S:]
-        shared_off, shared_h, shared_a = ctx.shared
         f = meta.ffn
         fs = meta.shared_ffn or f
         dout = x.new_zeros(T, h) if dout is None else dout.contiguous()
