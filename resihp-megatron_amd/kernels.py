@@ -1528,6 +1528,10 @@ def mx4_wgrad(a: Mx4, b: Mx4, offsets: torch.Tensor, out: torch.Tensor | None = 
     G = _mx4_offsets(offsets)
     _expect(a.rows is not None and (a.rows, a.groups) == (b.rows, b.groups) and a.groups == G,
             f"a and b must be quantised along their columns in the same {G} row groups")
+    # The kernel goes through as many places as the rows and groups ask for.
+    places = C.lib().rhp_mx4_padded_rows(a.rows, G)
+    _expect(a.length == b.length == places,
+            f"{a.rows} rows in {G} groups take {places} places, a and b have {a.length} and {b.length}")
     M, N = a.shape[0], b.shape[0]
     if out is None:
         out = torch.empty(G, M, N, dtype=torch.bfloat16, device=dev)

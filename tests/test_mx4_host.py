@@ -205,6 +205,17 @@ def test_python_entry_points_refuse_cpu_tensors_and_what_is_no_mx4():
             call()
 
 
+@pytest.mark.parametrize("length,rows,groups", [(128, 1000, 1), (1024, 1000, 2), (1152, 1000, 1), (128, 0, 1), (128, -5, 1)])
+def test_wgrad_refuses_matrices_whose_places_are_not_those_of_their_groups(length, rows, groups, monkeypatch):
+    """The kernel goes through the places that rows and groups ask for: codes of fewer would be read past their end."""
+    monkeypatch.setattr(K, "_need_cuda", lambda *ts: torch.device("cpu"))
+    monkeypatch.setattr(K, "_call", lambda *a: pytest.fail("a launch"))
+    q = K.Mx4(torch.zeros(8, length // 2, dtype=torch.uint8), torch.zeros(length // 128, 8, 4, dtype=torch.uint8), length, rows,
+              groups)
+    with pytest.raises(RuntimeError, match="places"):
+        K.mx4_wgrad(q, q, torch.zeros(groups + 1, dtype=torch.int32))
+
+
 def test_received_rows_do_not_run_in_4_bits_silently():
     for bits, msg in ((4, "model's dtype"), (8, "experts_bits must be")):
         runtime = SimpleNamespace(cfg=moe.MoEConfig(experts_bits=bits))
