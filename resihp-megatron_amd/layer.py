@@ -65,7 +65,7 @@ class LossTokens(NamedTuple):
 
 
 class RouterLosses(NamedTuple):
-    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads (not to be written before)."""
+    """Balance loss, z loss and the counts [S, E] they are made of, which the backward reads (unchanged until then)."""
 
     balance: torch.Tensor
     z: torch.Tensor
@@ -361,6 +361,7 @@ class _MoELayerFn(torch.autograd.Function):
         return outs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, _dcounts, d_balance=None, d_z=None, _dloss_counts=None):
         meta = ctx.meta
         T, h, P, G, S = ctx.dims

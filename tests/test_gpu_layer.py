@@ -446,3 +446,21 @@ def test_layer_error_leaves_bias_untouched():
     with pytest.raises(RuntimeError):
         moe.reference_forward(cfg, params, x)
     assert torch.equal(before, params["router.expert_bias"])
+
+
+@pytest.mark.parametrize("losses", [False, True])
+def test_layer_refuses_second_derivatives(losses):
+    """The backward's kernels are no part of a graph: a gradient's gradient is refused, not taken for zero."""
+    from resihp_megatron_amd.layer import LossTokens
+
+    say(f"second derivatives, losses {losses}")
+    cfg = moe.MoEConfig(device=DEV)
+    params = {k: moe.init_param(cfg, s).requires_grad_(s.trainable) for k, s in moe.moe_specs(cfg).items()}
+    fc1s, fc2s, *_ = moe._weights(cfg, params, range(cfg.num_experts))
+    x = moe.batch(cfg, 0)[0].requires_grad_(True)
+    outs = moe_layer(moe._layer_meta(cfg), x, params["router.weight"], None, fc1s, fc2s,
+                     losses=LossTokens() if losses else None)
+    total = outs[0].square().sum() + (outs[2].balance if losses else 0)
+    dx, = torch.autograd.grad(total, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (dx.square().sum() + x.sum()).backward()
