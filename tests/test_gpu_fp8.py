@@ -388,6 +388,52 @@ def test_fp8_layer_matches_quantized_emulation(case):
     assert rel_err(out, out_ref) <= LAYER_BAR
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_fp8_layer_with_losses(norm):
+    """The router's losses beside fp8 experts: alone their gradient is the bf16 layer's bit for bit, and it adds to the
+    experts'."""
+    from resihp_megatron_amd.fp8 import ACT, DH, DY, X, Fp8State
+    from resihp_megatron_amd.layer import LayerMeta, LossTokens, Norm, moe_layer
+
+    T, h, f, E, k = 200, 256, 256, 4, 2
+    say(f"fp8 layer with losses, norm {norm}")
+    x = seeded((T, h), 61, 1.0, torch.bfloat16).to(DEV).requires_grad_(True)
+    router = seeded((E, h), 62, 0.05, torch.float32).to(DEV).requires_grad_(True)
+    fc1 = [seeded((2 * f, h), 63 + e, 0.05, torch.bfloat16).to(DEV).requires_grad_(True) for e in range(E)]
+    fc2 = [seeded((h, f), 73 + e, 0.05, torch.bfloat16).to(DEV).requires_grad_(True) for e in range(E)]
+    dout = seeded((T, h), 64, 0.1, torch.bfloat16).to(DEV)
+    meta = LayerMeta(num_experts=E, top_k=k, ffn=f, act="swiglu")
+    mask = torch.arange(T, device=DEV) % 7 != 2
+    pre = Norm(torch.ones(h, device=DEV), torch.zeros(h, device=DEV)) if norm else None
+    leaves = [x, router, *fc1, *fc2]
+
+    def call(fp8, which):
+        st = None
+        if fp8:
+            st = Fp8State(E, 4, device=DEV)
+            st.seed_history({X: 4.0, ACT: 0.5, DY: 0.5, DH: 0.05, **{st.w1(e): 0.2 for e in range(E)},
+                             **{st.w2(e): 0.2 for e in range(E)}}, seed=8)
+        out, counts, *rest = moe_layer(meta, x, router, None, fc1, fc2, fp8=st, norm=pre,
+                                       losses=None if which == "out" else LossTokens(mask))
+        total = 0 if which == "losses" else (out * dout).sum()
+        if which != "out":
+            total = total + 3.0 * rest[0].balance + 2.0 * rest[0].z
+        return out, rest[0] if rest else None, torch.autograd.grad(total, leaves)
+
+    out, _, rows = call(True, "out")
+    same, losses, both = call(True, "both")
+    assert torch.equal(out, same)
+    _, _, alone = call(True, "losses")
+    _, want_losses, want = call(False, "losses")
+    assert torch.equal(losses.balance, want_losses.balance) and torch.equal(losses.counts, want_losses.counts)
+    assert torch.equal(alone[0], want[0]) and torch.equal(alone[1], want[1])
+    assert all((g == 0).all() for g in alone[2:])
+    # The router's gradient is a float sum of the two; x's rows (the norm's) are rounded to bf16 once more or less.
+    assert torch.equal(both[1], rows[1] + alone[1])
+    assert all(torch.equal(a, b) for a, b in zip(both[2:], rows[2:]))
+    assert rel_err(both[0], rows[0].double() + alone[0].double()) <= 2 ** -6
+
+
 def test_cast_many_equals_one_cast_per_tensor():
     """rhp_fp8_cast_many (the expert weights in one launch) gives every tensor the codes, amax and 1/scale
     of its own rhp_fp8_cast: tensors of different shapes, rows not a multiple of 128, an empty one."""
