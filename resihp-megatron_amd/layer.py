@@ -640,6 +640,7 @@ class _ExpertChunksFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy_recv):
         offsets, sort_row, xs, hpre, a, *ws = ctx.saved_tensors
         G = len(ws) // 2

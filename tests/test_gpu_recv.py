@@ -285,6 +285,19 @@ def test_config4_from_received_buffer(window):
     assert errs[worst] <= bar, errs
 
 
+def test_expert_outputs_refuse_second_derivatives():
+    cfg, recv, counts, src, w1, w2 = _ep_share(256, (0, 16))
+    rt, _ = _runtime(cfg, (0, 16), w1, w2)
+    full = np.zeros((8, 128), np.int64)
+    full[:, :16] = counts
+    say("received rows, second derivatives")
+    recv = recv.requires_grad_(True)
+    y = rt.expert_outputs(recv, torch.from_numpy(full))
+    drecv, = torch.autograd.grad(y.float().square().sum(), recv, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (drecv.float().square().sum() + recv.float().sum()).backward()
+
+
 def test_expert_outputs_reject_unhosted_expert():
     cfg, recv, counts, src, w1, w2 = _ep_share(256, (0, 16))
     rt, _ = _runtime(cfg, (0, 16), w1, w2)
