@@ -684,7 +684,8 @@ int rhp_fp8_gemm_cast(int epi, int G, const int32_t* offsets, const int32_t* pof
  * logits [T, E] RHP_F32 or RHP_F64, E <= 1024; topi [T, k], k <= 16; seq_offsets
  * [S+1] ascending token offsets, or NULL for one sequence of all tokens (S = 1); tokens
  * of no sequence do not count.  A row of logits that are all -inf adds nothing to
- * the sums.  No token at all: both losses are zero.
+ * the sums.  No token at all: both losses are zero.  Up to 2^20 sequences; one
+ * block joins their sums, 16 (of up to 64 experts) in some 3 us.
  * Writes balance and z (one value each, logits' type), counts [S, E] and tokens [S + 2]: n_s, then S'
  * and N.
  */
@@ -708,9 +709,9 @@ int rhp_router_loss_bwd(const void* d_balance, const void* d_z, const void* logi
  * gradient of all of them: dx [T, h] = dlogits W (x's type) and dw [E, h] =
  * dlogits^T x (the router's type); either may be NULL.  dlogits [T, E] and
  * router_w [E, h] are RHP_F64 iff x is, else RHP_F32; all tensors 16-byte
- * aligned; E <= 1024.  For bfloat16 x (h a multiple of 8) dx leaves out some
- * 2^-15 of |dlogits| |W| (its own rounding is 2^-9 of dx); infinities may come
- * out as NaN there.
+ * aligned; E <= 1024.  For bfloat16 x (h a multiple of 8) dx leaves out at most
+ * 2^-14 + 2^-15 of |dlogits| |W| (its own rounding is 2^-8 of dx); infinities may
+ * come out as NaN there.
  */
 size_t rhp_router_logits_bwd_workspace_bytes(int64_t T, int h, int E, int x_dtype);
 int rhp_router_logits_bwd(const void* dlogits, const void* x, int x_dtype, const void* router_w, int r_dtype,
@@ -789,7 +790,8 @@ int rhp_mx4_wgrad(int G, const int32_t* offsets, int64_t rows, int M, int N, con
  * w: G matrices of N rows with C = K (act RHP_ACT_SWIGLU: 2 N rows, gate rows
  * first, out = silu(gate) * up; RHP_ACT_GELU; -1: none).  N and K multiples of
  * 8.  The order of a row's sums is that of the sizes and of the groups' mean rows, whatever
- * the other rows hold.  Rows of no group are left as they are.
+ * the other rows hold: a row served alone and in a larger batch may differ in its last bit.
+ * Rows of no group are left as they are.
  */
 int rhp_mx4_rows_gemm(int G, const int32_t* offsets, int64_t rows, int N, int K, int act, const void* x,
                       const void* w_codes, const void* w_scales, void* out, hipStream_t stream);

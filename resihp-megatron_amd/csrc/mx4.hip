@@ -139,7 +139,8 @@ template <int kCtrl> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
 // once meet 64 banks; a thread then has whole blocks of a column and stores 16
 // bytes, four threads 64 of a line.  Bound by HBM: both directions of 8 x 28672 x 4096
 // bfloat16 557 us (2.9 GB, 5.2 TB/s), of 64 x 2816 x 2048 228, of 16384 x 28672 rows
-// 333 and of 16384 x 4096 40.5.  Tiles in plain order, whose neighbours' halves of a
+// 333 and of 16384 x 4096 40.5; 8 x 28672 x 4096 float32 906 (5.2 TB/s).  Rows alone, columns alone:
+// bfloat16 551, 453 us, float32 857, 799.  Tiles in plain order, whose neighbours' halves of a
 // line meet in no L2, take 702 and 369 us of the first and third.
 template <class S, bool kRows, bool kCols>
 __global__ __launch_bounds__(kQThreads) void mx4_quantize_kernel(Mx4QuantParams p) {

@@ -12,16 +12,18 @@
 // scales are exact; sums are float; the bfloat16 output is rounded once.
 //
 // A block computes 256 x 256 outputs on eight waves of 128 x 64; one block a CU.
-// Measured on 16384 rows of 8 groups: 28672 x 4096 in 1.22 ms (3.15 PFLOP/s), the
-// product back, 4096 x 28672, in 0.90 (4.26), the weights' gradient in 1.37 (2.81).
+// Measured on 16384 rows of 8 groups, of 2048 each / ragged (1356 to 4126): 28672 x
+// 4096 in 1.06 / 1.09 ms (3.6, 3.5 PFLOP/s), the product back, 4096 x 28672, in 0.91 /
+// 1.03 (4.2, 3.7), the weights' gradient in 1.32 / 1.35 (2.9, 2.8).
 // The matrix cores alone, on random codes in registers, hold 5.9 PFLOP/s of this
-// shape (9.2 on zeros: the clock falls with the power), and a further 4096 of K
-// costs 4.9 PFLOP/s; the rest is the first loads and the stores of a tile, which no
-// other block covers (without its stores 1.03 ms, without its loads 1.00).  Built
-// and timed against it on these three: blocks that walk their tiles with the next
-// one's loads under the stores, 16 x 16 x 128 products, four waves of 128 x 128 and
-// four stages of 128 places, none faster by more than 2 %; blocks that start at
-// different times, no difference.  Few rows take gg_mx4_short_kernel.
+// shape (9.2 on zeros: the clock falls with the power) and 7.25 of 16 x 16 x 128, and a
+// further 4096 of K runs at 4.9 PFLOP/s (ragged 4.6); the rest is the first loads and
+// the stores of a tile, which no other block covers (forward without its stores -16 %,
+// without its loads -18 %).  Built and timed against it on these three: blocks that walk
+// their tiles with the next one's loads under the stores, on either product, four waves
+// of 128 x 128 and four stages of 128 places, none faster by more than 2 %; blocks that
+// start at different times, no difference.  16 x 16 x 128 in this kernel's structure was
+// not built.  Few rows take gg_mx4_short_kernel.
 
 #include <type_traits>
 

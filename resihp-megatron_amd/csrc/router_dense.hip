@@ -12,8 +12,9 @@
 // operands are split into bfloat16 terms, v = t0 + t1 (+ t2) with t0 and t1 the
 // upper 8 bits of what is left (exact, by truncation) and the last rounded:
 //   dW  three terms of dl, all 24 bits, times x, which is bfloat16: exact products
-//   dx  two terms of dl and of W (the last rounded: 2^-17 of a factor left out), the product of
-//       the two small ones left out too: some 2^-15 of |dl| |W|, against the 2^-9 of dx's own rounding
+//   dx  two terms of dl and of W (the last rounded: 2^-16 of a factor left out at most), the
+//       product of the two small ones, each below 2^-7 of its factor, left out too: at most 2^-14 +
+//       2^-15 of |dl| |W|, against the 2^-8 of dx's own rounding
 // An infinite dl or W gives NaN (its second term is inf - inf).  Float32 and
 // float64 tokens, and rows that are not multiples of 8, take plain tiles of
 // fused multiply-adds.  dW is summed over slices of the tokens and then over the
@@ -39,7 +40,13 @@ constexpr int kChunkE = 64;        // experts that a dW block takes (128: its ac
 constexpr int kPlainTile = 64, kPlainK = 16, kPlainThreads = 256;
 
 // C[m, n] = sum_k A(m, k) B(k, n) over k in [k0, k1): 64 x 64 a block, 4 x 4 a thread.  kTransA: a is [K, M].
-// Bound by the fused multiply-adds and their reads from LDS.
+// Bound by the fused multiply-adds and their reads from LDS, eight for sixteen; dW has 64 experts a tile, however few
+// there are, and too few blocks where there are few.  us of dx, dW with the sum over the slices (a library product of the
+// same: dx, dW), where the tokens' bytes alone take 22, 90 and 45 in float32:
+//   16384 x 2048 by 64 experts    float32  93, 421 (60, 126)     float64 171, 563 (100, 1770)
+//   32768 x 4096 by 8                     163, 1796 (128, 280)           265, 2234 (180, 3546)
+//   32768 x 2048 by 128                   357, 1906 (171, 228)           652, 2380 (332, 3518)
+//   16384 x 2044 by 64, bfloat16 tokens    88, 429
 template <class A, class S, class O, bool kTransA>
 __global__ __launch_bounds__(kPlainThreads) void router_plain_kernel(const A* __restrict__ a, const S* __restrict__ b,
                                                                      int64_t M, int N, int64_t K, int64_t lda,
@@ -129,7 +136,8 @@ __device__ __forceinline__ void lds_sync() {
 // bytes.  More than 128 experts: W's terms are made again for every 64 tokens.
 // 16384 x 2048 by 64 experts 28 us (2.5 TB/s; a block's splits, products and stores follow
 // one another, two blocks a CU cover them), 16384 x 4096 by 8 experts 25 (5.4
-// TB/s), 32768 x 2048 by 128 experts 104 (the products' three terms).  Every wave with
+// TB/s), 32768 x 2048 by 128 experts 107 (the products' three terms; from 65 experts on the
+// block's 84 KB of LDS leave room for one a CU, so nothing covers them).  Every wave with
 // splits of its own took 64 us of the first.
 constexpr int kDxThreads = 256, kDxWaves = kDxThreads / 64, kDxTokens = 64;
 constexpr int kDxPitch = 72;   // halves a staged row of 64: 16-byte pieces, banks turned by 4 a row
